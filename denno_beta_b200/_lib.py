@@ -42,6 +42,13 @@ SIGNATURES = {
     "dnb_set_tc_min_tokens": (_i, [_vp, _i]),
     "dnb_set_router_tc": (_i, [_vp, _i]),
     "dnb_set_q4k_int": (_i, [_vp, _i]),
+    "dnb_mx4_bytes": (_i, [_i, _i, C.POINTER(_sz), C.POINTER(_sz)]),
+    "dnb_mx4_quantize_dev": (_i, [_vp, _i, _vp, _sz, _i, _i, _vp, _vp]),
+    "dnb_mx4_dequantize_dev": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _sz]),
+    "dnb_mx4_gemm_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
+    "dnb_mx4_gated_dev": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz]),
+    "dnb_gated_dev": (_i, [_vp, _i, _i, _vp, _sz, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "dnb_gated_backward_dev": (_i, [_vp, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _vp, _vp, _sz, _vp, _vp]),
     "dnb_moe_config": (_i, [_vp, _i, _i, _i, _i, _i, _i, _f, _i]),
     "dnb_register_experts": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _sz]),
     "dnb_register_router": (_i, [_vp, _i, _vp, _vp, _vp, _vp]),

@@ -1,0 +1,480 @@
+// Dense products on tcgen05: D[m][n] = sum_k A[m][k] B[n][k], stored as out[n][m] (m contiguous), for
+//   * 4-bit microscaled operands (kind::mxf4, 2^x scales of 32 elements taken from tensor memory) and 16-bit ones (kind::f16),
+//   * operands whose rows run along K, or (16 bit) along m or n, so that no gradient needs a transposed copy,
+//   * one A, or two with an accumulator each (gate and up) that the epilogue joins: act(g) * u.
+// m is the feature that is contiguous in the output: lane l of TMEM row quarter q holds m = 32 q + l, so that the stores of a column
+// are whole 64- or 128-byte lines without a trip through shared memory, a block of 32 features is one warp's column (the epilogue
+// can quantise), and few tokens make narrow tiles (n from 16) under full-height ones of weights.
+//
+// One CTA: warp 0 moves tiles by TMA through a ring of stages of 128 bytes of K a row, warp 1 issues the MMAs, eight warps read the
+// accumulators (two a row quarter).  Large outputs: one CTA per SM walks tiles, accumulators twice where TMEM has room, so that the
+// epilogue of a tile runs under the next one's MMAs.  Small outputs: a cluster splits K and its CTAs' partial sums are added through
+// distributed shared memory in ascending rank order (no workspace, no atomics: the same bits on every run).
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "dnb_common.cuh"
+#include "tc_ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace dnb {
+namespace dt {
+using namespace tcp;
+
+constexpr int TM = 128;             // rows of A in a tile
+constexpr int NTHREADS = 320;
+constexpr int EPI_WARPS = 8;
+constexpr int kWaitStage = 27, kWaitAcc = 28, kWaitDrain = 29;  // status codes of the waits
+
+enum Act { ACT_NONE = -1, ACT_SILU = 0, ACT_GELU = 1 };
+
+struct Params {
+    CUtensorMap a[2], b[2];
+    const uint8_t* sa[2];           // scale tiles of A (4 bit)
+    const uint8_t* sb;              // and of B
+    int M, N, K;
+    int passes;                     // 2: the sum goes on over a[1], b[1]
+    int both;                       // 2: twice the tiles, the second half with b[1] to out[1]
+    int tiles_m, tiles_n, splits;
+    int idesc_type;                 // 16 bit: 0 fp16, 1 bf16
+    int out_type, act;
+    void* out[2];
+    uint8_t* out_scales;            // MXFP4 results
+    float* pre;                     // gate and up before the activation [2][N][M], or null
+    size_t ldo;                     // elements between rows of out
+    int* status;
+};
+
+constexpr int pow2_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
+
+template <bool FP4_, int NA_, int BN_, bool AMN_ = false, bool BMN_ = false>
+struct Cfg {
+    static constexpr bool FP4 = FP4_, AMN = AMN_, BMN = BMN_;
+    static constexpr int NA = NA_, BN = BN_;
+    static constexpr int BK = FP4 ? 256 : 64;               // 128 bytes of a row
+    static constexpr int A_BYTES = TM * 128, B_BYTES = BN * 128;
+    static constexpr int SFA = FP4 ? 1024 : 0;              // scales of 128 rows x 256 elements
+    static constexpr int SFB_TILES = BN > 128 ? 2 : 1;
+    static constexpr int SFB = FP4 ? SFB_TILES * 1024 : 0;
+    static constexpr int STAGE = NA * A_BYTES + B_BYTES + NA * SFA + SFB;
+    static constexpr int PER_SM = BN < 128 ? 2 : 1;
+    static constexpr int BUDGET = PER_SM == 2 ? 115712 - 1536 : 232448 - 1536;
+    static constexpr int FIT = BUDGET / STAGE;
+    static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr int ACC = NA * BN;
+    static constexpr int SF_COLS = FP4 ? NA * 8 + SFB_TILES * 8 : 0;   // one of two buffers
+    static constexpr int BUFS = BN >= 128 && 2 * ACC + 2 * SF_COLS <= 512 ? 2 : 1;
+    static constexpr int COLS = pow2_cols(BUFS * ACC + 2 * SF_COLS);
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 512;
+    static_assert(STAGES >= 2 && PER_SM * COLS <= 512, "no room");
+    static_assert(!FP4 || (!AMN && !BMN), "4-bit operands lie along K");
+};
+
+__device__ __forceinline__ float act_of(int act, float g) {
+    if (act == ACT_SILU) return g / (1.f + __expf(-g));
+    const float t = tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g));
+    return 0.5f * g * (1.f + t);
+}
+
+template <int OUT>
+__device__ __forceinline__ void put(void* out, size_t at, float v) {
+    if constexpr (OUT == T_F32) reinterpret_cast<float*>(out)[at] = v;
+    else if constexpr (OUT == T_F16) reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+}
+
+// Byte of scale j (of 32 elements) of row r in the tiles of a matrix with `kb` tiles a row.
+__host__ __device__ __forceinline__ size_t scale_at(size_t r, int j, int kb) {
+    return ((r >> 7) * kb + (j >> 2)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + (j & 3);
+}
+// The scale byte of a block whose largest magnitude has these bits: floor(log2) - 2, at least 2^-127; 255 (NaN) where it is not finite.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+    const uint32_t ex = amax_bits >> 23;
+    return ex == 255 ? 255u : ex > 2 ? ex - 2 : 0u;
+}
+__device__ __forceinline__ float scale_inverse(uint32_t e) { return __uint_as_float((254u - (e == 255 ? 254u : e)) << 23); }  // 0 where the scale is NaN
+// Numbers as e2m1, the first in the lowest bits; nearest, ties to even, 6 beyond 6.
+__device__ __forceinline__ uint32_t e2m1_pair(float a, float b) {
+    uint16_t r;
+    asm("{\n\t.reg .b8 c;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\tmov.b16 %0, {c, c};\n\t}" : "=h"(r) : "f"(a), "f"(b));
+    return r & 0xffu;
+}
+__device__ __forceinline__ uint32_t e2m1_eight(const float (&v)[8], float by) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(v[0] * by), "f"(v[1] * by), "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by), "f"(v[7] * by));
+    return r;
+}
+
+// ---- tcgen05 of this file ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+}
+// 512 bytes of scales (32 x 16 bytes) to four TMEM columns of all four row quarters.
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem) {
+    const uint64_t desc = ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | ((smem >> 4) & 0x3FFFu);  // no swizzle, 8 rows of 16 bytes after 128
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(s32(dst)), "l"(src), "r"(bytes),
+                 "r"(s32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_float(uint32_t smem, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(smem), "r"(rank) : "memory");
+    return v;
+}
+
+struct Tile { int m, n, which; };
+template <class C>
+__device__ __forceinline__ Tile tile_of(const Params& p, int t) {
+    // Groups of 16 (8 with two A) rows of tiles, column by column: the tiles in flight read about as much of A as of B, and little of both.
+    constexpr int G = C::NA == 2 ? 8 : 16;
+    const int per = p.tiles_m * p.tiles_n;
+    Tile r;
+    r.which = t >= per;
+    if (r.which) t -= per;
+    const int g = t / (G * p.tiles_n), in = t - g * G * p.tiles_n, rows = min(G, p.tiles_m - g * G);
+    r.m = g * G + in % rows;
+    r.n = in / rows;
+    return r;
+}
+
+// One column of results: feature m of this lane (beyond M: nothing stored), row n of the output.
+template <class C, int OUT>
+__device__ __forceinline__ void emit(const Params& p, int which, int m, int n, float v0, float v1) {
+    float v = v0;
+    if constexpr (C::NA == 2) {
+        v = act_of(p.act, v0) * v1;
+        if (p.pre && m < p.M) {
+            p.pre[(size_t)n * p.M + m] = v0;
+            p.pre[((size_t)p.N + n) * p.M + m] = v1;
+        }
+    }
+    if constexpr (OUT == T_MXFP4) {
+        // The warp's 32 features are one block.
+        const int lane = threadIdx.x & 31;
+        const uint32_t e = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+        const float s = v * scale_inverse(e);
+        const float other = __shfl_xor_sync(0xffffffffu, s, 1);
+        uint32_t c = e == 255 ? 0u : (lane & 1) ? e2m1_pair(other, s) : e2m1_pair(s, other);
+        c <<= 8 * ((lane >> 1) & 3);
+        c |= __shfl_xor_sync(0xffffffffu, c, 2);
+        c |= __shfl_xor_sync(0xffffffffu, c, 4);
+        if (m < p.M && (lane & 7) == 0) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out[0]) + ((size_t)n * p.M + m) / 2) = c;
+        if (lane == 0) p.out_scales[scale_at(n, m >> 5, (p.M + 127) >> 7)] = (uint8_t)(m < p.M ? e : 0u);
+    } else {
+        if (m < p.M) put<OUT>(p.out[which], (size_t)n * p.ldo + m, v);
+    }
+}
+
+template <class C, int OUT>
+__device__ __forceinline__ void tile_out(const Params& p, const Tile& t, uint32_t tacc, int quad, int half, int lane) {
+    const int m = t.m * TM + quad * 32 + lane, n0 = t.n * C::BN;
+    const uint32_t ta = tacc + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+    for (int g = half; g < C::BN / 16; g += 2) {
+        uint32_t v0[16], v1[16];
+        tmem_ld16(ta + 16 * g, v0);
+        if constexpr (C::NA == 2) tmem_ld16(ta + C::BN + 16 * g, v1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int n = n0 + 16 * g + j;
+            if (n < p.N) emit<C, OUT>(p, t.which, m, n, __uint_as_float(v0[j]), C::NA == 2 ? __uint_as_float(v1[j]) : 0.f);
+        }
+    }
+}
+
+template <class C, int OUT>
+__device__ __forceinline__ void split_out(const Params& p, const Tile& t, uint32_t red, uint32_t rank, int quad, int half, int lane) {
+    const int m = t.m * TM + quad * 32 + lane, n0 = t.n * C::BN;
+    for (int c = (int)rank + p.splits * half; c < C::BN && n0 + c < p.N; c += 2 * p.splits) {
+        float s0 = 0.f, s1 = 0.f;
+        for (int r = 0; r < p.splits; ++r) {
+            s0 += peer_float(red + 4u * (uint32_t)(c * TM + quad * 32 + lane), r);
+            if constexpr (C::NA == 2) s1 += peer_float(red + 4u * (uint32_t)((C::BN + c) * TM + quad * 32 + lane), r);
+        }
+        emit<C, OUT>(p, t.which, m, n0 + c, s0, s1);
+    }
+}
+
+template <class C>
+__global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid_constant__ Params p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* tfull = empty + C::STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < C::STAGES; ++i) {
+            mb_init(&full[i], 1);
+            mb_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mb_init(&tfull[i], 1);
+            mb_init(&tempty[i], EPI_WARPS);
+        }
+        fence_mbarrier_init();
+    }
+    if (warp == 1) tmem_alloc<C::COLS>(tmem_slot);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const int kch = (p.K + C::BK - 1) / C::BK, chunks = kch * p.passes;
+    const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+    const int c0 = (int)((long long)chunks * rank / p.splits), c1 = (int)((long long)chunks * (rank + 1) / p.splits);
+    const int tiles = p.tiles_m * p.tiles_n * p.both;
+    const int first = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, step = p.splits > 1 ? tiles : gridDim.x;
+    const int nkb = (p.K + 127) >> 7;  // scale tiles along K
+    bool ok = true;
+
+    if (warp == 0) {
+        // ---------------- TMA ----------------
+        int it = 0;
+        for (int t = first; t < tiles && ok; t += step) {
+            const Tile tl = tile_of<C>(p, t);
+            const int m0 = tl.m * TM, n0 = tl.n * C::BN;
+            for (int c = c0; c < c1; ++c, ++it) {
+                const int st = it % C::STAGES, n = it / C::STAGES;
+                if (n > 0) ok = warp_all(mb_wait(&empty[st], (uint32_t)(n - 1) & 1u, p.status, kWaitStage));
+                if (!ok) break;
+                if (elect_one()) {
+                    uint8_t* s = smem + st * C::STAGE;
+                    const int pass = c >= kch, kc = pass ? c - kch : c;
+                    int kbs = 0, bt = 0;
+                    if constexpr (C::FP4) {
+                        kbs = min(2, nkb - 2 * kc);
+                        bt = min(C::SFB_TILES, ((p.N + 127) >> 7) - (n0 >> 7));
+                    }
+                    mb_expect_tx(&full[st], (uint32_t)(C::NA * C::A_BYTES + C::B_BYTES + (C::NA + bt) * kbs * 512));
+#pragma unroll
+                    for (int a = 0; a < C::NA; ++a) {
+                        const CUtensorMap* map = &p.a[C::NA == 2 ? a : pass];
+                        if constexpr (C::AMN) {
+#pragma unroll
+                            for (int i = 0; i < TM / 64; ++i) tma_load_2d(s + a * C::A_BYTES + i * 8192, map, m0 + 64 * i, kc * 64, &full[st]);
+                        } else {
+                            tma_load_2d(s + a * C::A_BYTES, map, kc * (C::FP4 ? 128 : 64), m0, &full[st]);
+                        }
+                    }
+                    uint8_t* sb = s + C::NA * C::A_BYTES;
+                    const CUtensorMap* map = &p.b[pass | tl.which];
+                    if constexpr (C::BMN) {
+#pragma unroll
+                        for (int i = 0; i < C::BN / 64; ++i) tma_load_2d(sb + i * 8192, map, n0 + 64 * i, kc * 64, &full[st]);
+                    } else {
+                        tma_load_2d(sb, map, kc * (C::FP4 ? 128 : 64), n0, &full[st]);
+                    }
+                    if constexpr (C::FP4) {
+                        uint8_t* sf = sb + C::B_BYTES;
+                        for (int a = 0; a < C::NA; ++a)
+                            bulk_load(sf + a * 1024, p.sa[a] + ((size_t)tl.m * nkb + 2 * kc) * 512, kbs * 512, &full[st]);
+                        for (int i = 0; i < bt; ++i)
+                            bulk_load(sf + (C::NA + i) * 1024, p.sb + ((size_t)((n0 >> 7) + i) * nkb + 2 * kc) * 512, kbs * 512, &full[st]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok)  // copies in flight end before their shared memory is given up
+            for (int i = max(0, it - C::STAGES); i < it; ++i) mb_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
+    } else if (warp == 1) {
+        // ---------------- MMA issue ----------------
+        const uint32_t smem_lo = s32(smem) >> 4;
+        constexpr uint32_t LA = (C::AMN ? (8192u >> 4) : 1u) << 16, LB = (C::BMN ? (8192u >> 4) : 1u) << 16;
+        constexpr uint32_t KA = C::AMN ? 128 : 2, KB = C::BMN ? 128 : 2;  // bytes / 16 from one K step of an MMA to the next
+        const uint32_t sf_tmem = tmem + C::BUFS * C::ACC;
+        uint32_t idesc;
+        if constexpr (C::FP4)  // e2m1 operands, 2^x scales
+            idesc = (1u << 7) | (1u << 10) | ((uint32_t)(C::BN >> 3) << 17) | (1u << 23) | (1u << 27);
+        else
+            idesc = (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) | ((uint32_t)C::BMN << 16) |
+                    ((uint32_t)(C::BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+        int it = 0, nt = 0;
+        for (int t = first; t < tiles && ok; t += step, ++nt) {
+            const int buf = nt % C::BUFS, use = nt / C::BUFS;
+            if (use > 0) ok = warp_all(mb_wait(&tempty[buf], (uint32_t)(use - 1) & 1u, p.status, kWaitDrain));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + buf * C::ACC;
+            const int n_sf = C::FP4 ? ((tile_of<C>(p, t).n * C::BN) & 127) >> 5 : 0;  // narrow tiles start inside a tile of scales
+            for (int c = c0; c < c1; ++c, ++it) {
+                const int st = it % C::STAGES, n = it / C::STAGES;
+                ok = warp_all(mb_wait(&full[st], (uint32_t)n & 1u, p.status, kWaitStage));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a0 = smem_lo + (uint32_t)(st * (C::STAGE >> 4)), b0 = a0 + ((C::NA * C::A_BYTES) >> 4);
+                    if constexpr (C::FP4) {
+                        const uint32_t sf = b0 + (C::B_BYTES >> 4), ts = sf_tmem + (it & 1) * C::SF_COLS;
+                        const int left = p.K - c * C::BK, kbs = left > 128 ? 2 : 1, steps = left >= C::BK ? 4 : (left + 63) >> 6;
+                        // TMEM: A's scales 4 columns per (A, 128 of K), B's 4 per (128 of K, 128 rows)
+                        for (int kb = 0; kb < kbs; ++kb) {
+#pragma unroll
+                            for (int a = 0; a < C::NA; ++a) scales_to_tmem(ts + a * 8 + kb * 4, (sf + a * 64 + kb * 32) << 4);
+#pragma unroll
+                            for (int i = 0; i < C::SFB_TILES; ++i)
+                                scales_to_tmem(ts + C::NA * 8 + (kb * C::SFB_TILES + i) * 4, (sf + (C::NA + i) * 64 + kb * 32) << 4);
+                        }
+                        for (int ks = 0; ks < steps; ++ks) {
+                            const uint32_t id = idesc | ((uint32_t)(ks & 1) << 30) | ((uint32_t)(ks & 1) << 5);  // scales 0, 1 or 2, 3 of a word
+                            const uint32_t tb = ts + C::NA * 8 + (ks >> 1) * C::SFB_TILES * 4 + n_sf;
+#pragma unroll
+                            for (int a = 0; a < C::NA; ++a)
+                                mma_mxf4(d + a * C::BN, desc_of((a0 + a * (C::A_BYTES >> 4) + ks * KA) & 0x3FFFu | LA), desc_of((b0 + ks * KB) & 0x3FFFu | LB), id,
+                                         ts + a * 8 + (ks >> 1) * 4, tb, c > c0 || ks > 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                            for (int a = 0; a < C::NA; ++a)
+                                mma_bf16(d + a * C::BN, desc_of((a0 + a * (C::A_BYTES >> 4) + ks * KA) & 0x3FFFu | LA), desc_of((b0 + ks * KB) & 0x3FFFu | LB), idesc,
+                                         c > c0 || ks > 0);
+                    }
+                    mma_commit(&empty[st]);
+                    if (c == c1 - 1) mma_commit(&tfull[buf]);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ---------------- epilogue ----------------
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        int nt = 0;
+        for (int t = first; t < tiles && ok; t += step, ++nt) {
+            const int buf = nt % C::BUFS, use = nt / C::BUFS;
+            ok = warp_all(mb_wait(&tfull[buf], (uint32_t)use & 1u, p.status, kWaitAcc));
+            if (!ok) break;
+            tc_fence_after();
+            const Tile tl = tile_of<C>(p, t);
+            const uint32_t tacc = tmem + buf * C::ACC;
+            if (p.splits == 1) {
+                switch (p.out_type) {
+                    case T_F32: tile_out<C, T_F32>(p, tl, tacc, quad, half, lane); break;
+                    case T_F16: tile_out<C, T_F16>(p, tl, tacc, quad, half, lane); break;
+                    case T_BF16: tile_out<C, T_BF16>(p, tl, tacc, quad, half, lane); break;
+                    default: if constexpr (C::FP4 && C::NA == 2) tile_out<C, T_MXFP4>(p, tl, tacc, quad, half, lane);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&tempty[buf]);
+            } else {
+                // This CTA's share of the sum, into the ring's memory: all copies have landed and been read.
+                float* red = reinterpret_cast<float*>(smem);
+                const uint32_t ta = tacc + ((uint32_t)(quad * 32) << 16);
+                for (int g = half; g < C::ACC / 16; g += 2) {
+                    uint32_t v[16];
+                    tmem_ld16(ta + 16 * g, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) red[(16 * g + j) * TM + quad * 32 + lane] = __uint_as_float(v[j]);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (p.splits > 1) {
+        cluster_sync();
+        if (warp >= 2) {
+            const int quad = warp & 3, half = (warp - 2) >> 2;
+            const Tile tl = tile_of<C>(p, first);
+            const uint32_t red = s32(smem);
+            switch (p.out_type) {
+                case T_F32: split_out<C, T_F32>(p, tl, red, rank, quad, half, lane); break;
+                case T_F16: split_out<C, T_F16>(p, tl, red, rank, quad, half, lane); break;
+                case T_BF16: split_out<C, T_BF16>(p, tl, red, rank, quad, half, lane); break;
+                default: if constexpr (C::FP4 && C::NA == 2) split_out<C, T_MXFP4>(p, tl, red, rank, quad, half, lane);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // nobody leaves while its sums are being read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free<C::COLS>(tmem);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------
+struct Operand {  // a matrix in memory
+    const void* data;
+    uint64_t rows, cols, pitch;  // pitch: bytes between rows
+};
+template <class C>
+int operand_map(CUtensorMap* m, const Operand& o, int box_rows, int type) {
+    if constexpr (C::FP4) return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.data, o.rows, o.cols / 2, o.pitch, box_rows);
+    return tiled_map(m, type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.data, o.rows, o.cols, o.pitch, box_rows);
+}
+
+// p: everything but the maps and the tiles.  a, b: C::NA or p.passes operands of A, p.passes or p.both of B.
+template <class C>
+int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* b, int nb, int type, const char* name) {
+    int rc;
+    for (int i = 0; i < na; ++i)
+        if ((rc = operand_map<C>(&p.a[i], a[i], C::AMN ? 64 : TM, type))) return rc;
+    for (int i = 0; i < nb; ++i)
+        if ((rc = operand_map<C>(&p.b[i], b[i], C::BMN ? 64 : C::BN, type))) return rc;
+    p.idesc_type = type == T_BF16;
+    p.status = c->status;
+    p.tiles_m = (p.M + TM - 1) / TM;
+    p.tiles_n = (p.N + C::BN - 1) / C::BN;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.both, chunks = (int64_t)((p.K + C::BK - 1) / C::BK) * p.passes;
+    if (tiles > 0x3fffffff) {
+        set_error("%s: %d x %d results are more than one launch takes", name, p.N, p.M);
+        return DNB_DECLINED;
+    }
+    static_assert(C::ACC * TM * 4 <= C::STAGES * C::STAGE, "the partial sums of a split lie in the ring");
+    const int slots = c->sm_count * C::PER_SM;
+    p.splits = 1;
+    while (p.splits < 8 && tiles * p.splits * 2 <= slots && chunks >= p.splits * 2) p.splits *= 2;
+    const unsigned grid = p.splits > 1 ? (unsigned)(tiles * p.splits) : (unsigned)(tiles < slots ? tiles : slots);
+    static SmemGrant grant;
+    DNB_CUDA(grant_smem(grant, c->device, dense_kernel<C>, C::SMEM));
+    ProfScope prof_(c, c->stream, name);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(NTHREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = c->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = c->use_pdl;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = p.splits;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.splits > 1 ? 2 : 1;
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, dense_kernel<C>, p));
+    c->launches++;
+    return DNB_OK;
+}
+
+}  // namespace dt
+}  // namespace dnb

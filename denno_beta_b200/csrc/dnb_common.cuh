@@ -22,6 +22,8 @@ constexpr int T_F32 = 0, T_Q5_1 = 7, T_Q8_0 = 8, T_Q4_K = 12, T_Q5_K = 13, T_Q6_
 // The block types of real checkpoints' remaining tensors (exp_iq.rs:390-400, cuda.rs:7364-7373):
 // served by the tiled kernels and the sequential checker, not by the decode fast kernels.
 constexpr int T_Q4_0 = 2, T_IQ4_NL = 20, T_IQ3_S = 21, T_IQ2_S = 22, T_IQ4_XS = 23, T_Q2_0 = 42;
+// Types of dense operands (mx4.cu, gated.cu); no block format of a registered matrix.
+constexpr int T_F16 = 1, T_BF16 = 30, T_MXFP4 = 39;
 
 __host__ __device__ constexpr int type_size(int t) {
     return t == T_Q4_K ? 144 : t == T_IQ3_XXS ? 98 : t == T_Q6_K ? 210 : t == T_Q8_0 ? 34 : t == T_Q5_K ? 176

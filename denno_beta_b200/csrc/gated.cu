@@ -1,0 +1,204 @@
+// The gated feed-forward block on 16-bit operands: out = act(x G^T) * (x U^T), both projections, the activation and the product in one
+// kernel, and its backward pass (dense_tc.cuh).
+//
+//   g = x G^T, u = x U^T, out = act(g) u
+//   du = dout act(g),  dg = dout u act'(g)                      gradients_kernel
+//   dx = dg G + du U                                            one launch: the sum over features goes on from gate to up
+//   dG = dg^T x,  dU = du^T x                                   one launch: two outputs
+// No operand is transposed in memory: the tensor core takes G, U, x, dg and du from shared memory with either index innermost.
+// Kept from the forward pass are g and u, in 32 bits: rounded to 16, dg and du would be off by twice their own rounding.
+// dg and du are rounded to the operands' type, as the tensor cores take them; all sums are 32 bits.
+#include "dense_tc.cuh"
+
+namespace dnb {
+namespace gt {
+using namespace dt;
+
+__device__ __forceinline__ void act_and_slope(int act, float g, float& a, float& slope) {
+    if (act == ACT_SILU) {
+        const float p = 1.f / (1.f + __expf(-g));
+        a = g * p;
+        slope = p * (1.f + g * (1.f - p));
+    } else {
+        const float t = tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g));
+        a = 0.5f * g * (1.f + t);
+        slope = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * 0.7978845608028654f * (1.f + 0.134145f * g * g);
+    }
+}
+
+// Eight features a thread: pre [2][nt][n] fp32, dout rows ldd apart, dpre [2][nt][n].
+template <int T>
+__global__ void __launch_bounds__(256)
+gradients_kernel(int act, const float* __restrict__ pre, const void* __restrict__ dout, size_t ldd, int nt, int n, void* __restrict__ dpre) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const size_t per = n / 8, all = per * nt, plane = (size_t)nt * n;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+        const size_t t = i / per, at = (i - t * per) * 8;
+        float g[8], u[8];
+        const float4* gp = reinterpret_cast<const float4*>(pre + t * n + at);
+        const float4* up = reinterpret_cast<const float4*>(pre + plane + t * n + at);
+        *reinterpret_cast<float4*>(g) = gp[0];
+        *reinterpret_cast<float4*>(g + 4) = gp[1];
+        *reinterpret_cast<float4*>(u) = up[0];
+        *reinterpret_cast<float4*>(u + 4) = up[1];
+        const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dout) + t * ldd + at);
+        uint4 og, ou;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint16_t b = reinterpret_cast<const uint16_t*>(&raw)[j];
+            const float d = T == T_BF16 ? __bfloat162float(__ushort_as_bfloat16(b)) : __half2float(__ushort_as_half(b));
+            float a, slope;
+            act_and_slope(act, g[j], a, slope);
+            put<T>(&og, j, d * u[j] * slope);
+            put<T>(&ou, j, d * a);
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dpre) + t * n + at) = og;
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dpre) + plane + t * n + at) = ou;
+    }
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The checks that both directions share: type, activation, sizes.
+static int check_shape(const char* what, int act, int type, int nt, int k, int n) {
+    if (nt < 0 || k < 1 || n < 1 || (act != ACT_SILU && act != ACT_GELU)) {
+        set_error("%s: bad argument (activation %d, tokens %d, k %d, n %d)", what, act, nt, k, n);
+        return DNB_ERR_ARG;
+    }
+    if ((type != T_F16 && type != T_BF16) || k % 8 || n % 8) {
+        set_error("%s: ggml type %d with k=%d, n=%d is not handled (F16 or BF16, multiples of 8)", what, type, k, n);
+        return DNB_DECLINED;
+    }
+    return DNB_OK;
+}
+// Rows of a matrix that TMA or 16-byte loads take.
+static int check_rows(const char* what, const char* name, const void* p, size_t ld, int cols) {
+    if (!p || ld < (size_t)cols) {
+        set_error("%s: %s is missing, or its rows of %d are %zu apart", what, name, cols, ld);
+        return DNB_ERR_ARG;
+    }
+    if (!aligned16(p) || ld % 8) {
+        set_error("%s: rows of %s start at multiples of 16 bytes", what, name);
+        return DNB_DECLINED;
+    }
+    return DNB_OK;
+}
+
+}  // namespace gt
+}  // namespace dnb
+
+using namespace dnb;
+using namespace dnb::gt;
+
+extern "C" {
+
+int dnb_gated_dev(dnb_ctx* c, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev, int nt, int k, int n, void* out_dev,
+                  size_t ldo, float* pre_dev) {
+    if (!c) return DNB_ERR_ARG;
+    int rc = check_shape("gated", act, type, nt, k, n);
+    if (rc || nt == 0) return rc;
+    if ((rc = check_rows("gated", "x", x_dev, ldx, k))) return rc;
+    if ((rc = check_rows("gated", "gate", gate_dev, k, k))) return rc;
+    if ((rc = check_rows("gated", "up", up_dev, k, k))) return rc;
+    if (!out_dev || ldo < (size_t)n) {
+        set_error("gated: out is missing, or its rows of %d are %zu apart", n, ldo);
+        return DNB_ERR_ARG;
+    }
+    if ((uintptr_t)out_dev % 2 || !aligned16(pre_dev)) {
+        set_error("gated: misaligned out or pre");
+        return DNB_DECLINED;
+    }
+    DNB_CUDA(cudaSetDevice(c->device));
+    Params p = {};
+    p.M = n; p.N = nt; p.K = k;
+    p.passes = p.both = 1;
+    p.out[0] = out_dev;
+    p.out_type = type;
+    p.ldo = ldo;
+    p.act = act;
+    p.pre = pre_dev;
+    const Operand a[2] = {{gate_dev, (uint64_t)n, (uint64_t)k, (uint64_t)k * 2}, {up_dev, (uint64_t)n, (uint64_t)k, (uint64_t)k * 2}};
+    const Operand b = {x_dev, (uint64_t)nt, (uint64_t)k, (uint64_t)ldx * 2};
+    if (nt <= 16) return launch_dense<Cfg<false, 2, 16>>(c, p, a, 2, &b, 1, type, "gated");
+    if (nt <= 32) return launch_dense<Cfg<false, 2, 32>>(c, p, a, 2, &b, 1, type, "gated");
+    if (nt <= 64) return launch_dense<Cfg<false, 2, 64>>(c, p, a, 2, &b, 1, type, "gated");
+    return launch_dense<Cfg<false, 2, 128>>(c, p, a, 2, &b, 1, type, "gated");
+}
+
+int dnb_gated_backward_dev(dnb_ctx* c, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev, const float* pre_dev,
+                           const void* dout_dev, size_t ldd, int nt, int k, int n, void* dpre_dev, void* dx_dev, size_t lddx, void* dgate_dev, void* dup_dev) {
+    if (!c) return DNB_ERR_ARG;
+    int rc = check_shape("gated_backward", act, type, nt, k, n);
+    if (rc) return rc;
+    const bool weights = dgate_dev || dup_dev;
+    if (weights && (!dgate_dev || !dup_dev)) {
+        set_error("gated_backward: gradients of both weights, or of none");
+        return DNB_ERR_ARG;
+    }
+    if ((uintptr_t)dgate_dev % 2 || (uintptr_t)dup_dev % 2 || (uintptr_t)dx_dev % 2) {
+        set_error("gated_backward: misaligned result");
+        return DNB_DECLINED;
+    }
+    if (nt > 0) {
+        if ((rc = check_rows("gated_backward", "dout", dout_dev, ldd, n))) return rc;
+        if ((rc = check_rows("gated_backward", "pre", pre_dev, n, n))) return rc;
+        if ((rc = check_rows("gated_backward", "dpre", dpre_dev, n, n))) return rc;
+        if (weights && (rc = check_rows("gated_backward", "x", x_dev, ldx, k))) return rc;
+        if (dx_dev && ((rc = check_rows("gated_backward", "gate", gate_dev, k, k)) || (rc = check_rows("gated_backward", "up", up_dev, k, k)))) return rc;
+        if (dx_dev && lddx < (size_t)k) {
+            set_error("gated_backward: rows of %d of dx are %zu apart", k, lddx);
+            return DNB_ERR_ARG;
+        }
+    }
+    DNB_CUDA(cudaSetDevice(c->device));
+    if (nt == 0) {  // sums of nothing
+        if (weights) {
+            DNB_CUDA(cudaMemsetAsync(dgate_dev, 0, (size_t)n * k * 2, c->stream));
+            DNB_CUDA(cudaMemsetAsync(dup_dev, 0, (size_t)n * k * 2, c->stream));
+        }
+        return DNB_OK;
+    }
+    const size_t groups = (size_t)nt * n / 8, want = (groups + 255) / 256, most = (size_t)c->sm_count * 8;
+    {
+        ProfScope prof_(c, c->stream, "gated_gradients");
+        const dim3 grid((unsigned)(want < most ? want : most));
+        if (type == T_BF16) DNB_CUDA(launch_k(gradients_kernel<T_BF16>, grid, dim3(256), 0, c->stream, c->use_pdl, act, pre_dev, dout_dev, ldd, nt, n, dpre_dev));
+        else DNB_CUDA(launch_k(gradients_kernel<T_F16>, grid, dim3(256), 0, c->stream, c->use_pdl, act, pre_dev, dout_dev, ldd, nt, n, dpre_dev));
+        c->launches++;
+    }
+    const uint8_t* dpre = (const uint8_t*)dpre_dev;
+    const uint64_t N = n, K = k, T = nt;
+    const Operand d[2] = {{dpre, T, N, N * 2}, {dpre + T * N * 2, T, N, N * 2}};
+    if (dx_dev) {
+        Params p = {};
+        p.M = k; p.N = nt; p.K = n;
+        p.passes = 2;
+        p.both = 1;
+        p.out[0] = dx_dev;
+        p.out_type = type;
+        p.ldo = lddx;
+        const Operand w[2] = {{gate_dev, N, K, K * 2}, {up_dev, N, K, K * 2}};
+        if (nt <= 16) rc = launch_dense<Cfg<false, 1, 16, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        else if (nt <= 32) rc = launch_dense<Cfg<false, 1, 32, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        else if (nt <= 64) rc = launch_dense<Cfg<false, 1, 64, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        else if (nt <= 128) rc = launch_dense<Cfg<false, 1, 128, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        else rc = launch_dense<Cfg<false, 1, 256, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        if (rc) return rc;
+    }
+    if (weights) {
+        Params p = {};
+        p.M = k; p.N = n; p.K = nt;
+        p.passes = 1;
+        p.both = 2;
+        p.out[0] = dgate_dev;
+        p.out[1] = dup_dev;
+        p.out_type = type;
+        p.ldo = k;
+        const Operand x = {x_dev, T, K, (uint64_t)ldx * 2};
+        if ((rc = launch_dense<Cfg<false, 1, 256, true, true>>(c, p, &x, 1, d, 2, type, "gated_dw"))) return rc;
+    }
+    return DNB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,44 @@
+// TMA tensor maps of row-major matrices (host side).
+#pragma once
+#include <cuda.h>
+
+#include "dnb_common.cuh"
+
+namespace dnb {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return ok ? (EncodeTiledFn)p : (EncodeTiledFn) nullptr;
+    }();
+    return fn;
+}
+
+// [rows][cols] of `type`, rows `pitch` bytes apart, in boxes of 128 bytes x box_rows with the 128-byte swizzle; zeros beyond the matrix.
+inline int tiled_map(CUtensorMap* m, CUtensorMapDataType type, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch,
+                     uint32_t box_rows) {
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) {
+        set_error("cuTensorMapEncodeTiled is not available from this driver");
+        return DNB_ERR_CUDA;
+    }
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / elem_bytes), box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d) for %llu x %llu box %u", (int)r, (unsigned long long)rows, (unsigned long long)cols, box_rows);
+        return DNB_ERR_CUDA;
+    }
+    return DNB_OK;
+}
+
+}  // namespace dnb

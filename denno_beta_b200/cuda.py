@@ -16,6 +16,9 @@ from ._lib import DnbError, check
 # ggml type ids (kquant.rs:72-104)
 Q5_1, Q8_0, Q4_K, Q5_K, Q6_K, IQ3_XXS = 7, 8, 12, 13, 14, 18
 Q4_0, IQ4_NL, IQ3_S, IQ2_S, IQ4_XS, Q2_0 = 2, 20, 21, 22, 23, 42
+# types of the dense operators (mx4_*, gated_*), and their activations
+F32, F16, BF16, MXFP4 = 0, 1, 30, 39
+ACT_SILU, ACT_GELU = 0, 1
 GATE, UP, DOWN, SHARED_GATE, SHARED_UP, SHARED_DOWN = range(6)
 
 TYPE_SIZE = {Q5_1: 24, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210, IQ3_XXS: 98,
@@ -29,6 +32,14 @@ def row_bytes(ty, n_in):
     if ty not in TYPE_SIZE or n_in <= 0 or n_in % BLOCK_ELEMS[ty]:
         raise ValueError("n_in=%d is not a whole number of blocks of ggml type %d" % (n_in, ty))
     return n_in // BLOCK_ELEMS[ty] * TYPE_SIZE[ty]
+
+
+def mx4_bytes(rows, k):
+    """Bytes of the codes and of the scales of a microscaled 4-bit matrix [rows][k]; None when k is not a multiple of 32."""
+    codes, scales = C.c_size_t(), C.c_size_t()
+    if not check(_lib.load().dnb_mx4_bytes(rows, k, C.byref(codes), C.byref(scales)), True):
+        return None
+    return codes.value, scales.value
 
 
 def _p(a):
@@ -178,6 +189,36 @@ class CudaCtx:
     def set_router_tc(self, on):
         """Router logits of calls of 16 tokens or more: tcgen05 kernel (default) or the fp32 FMA kernel."""
         check(self.lib.dnb_set_router_tc(self.h, int(on)))
+
+    # -- microscaled 4-bit matrices (device pointers; see dnb200.h for the layout) ----------
+    # Row distances (ld*, in elements) default to rows without a gap.  False = declined.
+    def mx4_quantize_dev(self, ty, x_ptr, rows, k, codes_ptr, scales_ptr, ldx=0):
+        """Rows of type F32, F16, BF16, or MXFP4 (a GGUF file's blocks) to codes and scales."""
+        return check(self.lib.dnb_mx4_quantize_dev(self.h, ty, x_ptr, ldx or k, rows, k, codes_ptr, scales_ptr), True)
+
+    def mx4_dequantize_dev(self, codes_ptr, scales_ptr, rows, k, ty, out_ptr, ldo=0):
+        """Codes and scales to the numbers that they stand for, F32, F16 or BF16."""
+        return check(self.lib.dnb_mx4_dequantize_dev(self.h, codes_ptr, scales_ptr, rows, k, ty, out_ptr, ldo or k), True)
+
+    def mx4_gemm_dev(self, x_codes, x_scales, w_codes, w_scales, nt, k, n, ty, out_ptr, ldo=0):
+        """out[nt, n] = X[nt, k] W[n, k]^T, both in 4 bits; out F32, F16 or BF16."""
+        return check(self.lib.dnb_mx4_gemm_dev(self.h, x_codes, x_scales, w_codes, w_scales, nt, k, n, ty, out_ptr, ldo or n), True)
+
+    def mx4_gated_dev(self, act, x_codes, x_scales, gate_codes, gate_scales, up_codes, up_scales, nt, k, n, ty, out_ptr, out_scales=None, ldo=0):
+        """out[nt, n] = act(X gate^T) * (X up^T), all in 4 bits; out F32, F16 or BF16, or MXFP4: codes to out_ptr, scales to out_scales."""
+        return check(self.lib.dnb_mx4_gated_dev(self.h, act, x_codes, x_scales, gate_codes, gate_scales, up_codes, up_scales, nt, k, n, ty, out_ptr,
+                                                out_scales, ldo or n), True)
+
+    # -- gated feed-forward block on F16 or BF16 operands (device pointers) -------------------
+    def gated_dev(self, act, ty, x_ptr, gate_ptr, up_ptr, nt, k, n, out_ptr, pre_ptr=None, ldx=0, ldo=0):
+        """out[nt, n] = act(x gate^T) * (x up^T); pre_ptr: fp32 [2, nt, n], kept for the backward pass."""
+        return check(self.lib.dnb_gated_dev(self.h, act, ty, x_ptr, ldx or k, gate_ptr, up_ptr, nt, k, n, out_ptr, ldo or n, pre_ptr), True)
+
+    def gated_backward_dev(self, act, ty, x_ptr, gate_ptr, up_ptr, pre_ptr, dout_ptr, nt, k, n, dpre_ptr, dx_ptr=None, dgate_ptr=None, dup_ptr=None,
+                           ldx=0, ldd=0, lddx=0):
+        """Gradients of x (dx_ptr, or None) and of both weights (or None) from pre and the gradient of out; dpre_ptr: [2, nt, n] of the type."""
+        return check(self.lib.dnb_gated_backward_dev(self.h, act, ty, x_ptr, ldx or k, gate_ptr, up_ptr, pre_ptr, dout_ptr, ldd or n, nt, k, n, dpre_ptr,
+                                                     dx_ptr, lddx or k, dgate_ptr, dup_ptr), True)
 
     # -- MoE model ----------------------------------------------------------------
     def moe_config(self, n_layer, n_embd, n_ff, n_expert, n_expert_used, n_shared_ff=0, rms_eps=1e-6,

@@ -53,6 +53,12 @@ extern "C" {
 #define DNB_GGML_IQ2_S 22
 #define DNB_GGML_IQ4_XS 23
 #define DNB_GGML_Q2_0 42
+/* Types of the dense operators below (kquant.rs:72-104 gives the ids); MXFP4 as a file holds it, or the layout
+ * of dnb_mx4_quantize_dev where the declaration says so. */
+#define DNB_GGML_F32 0
+#define DNB_GGML_F16 1
+#define DNB_GGML_BF16 30
+#define DNB_GGML_MXFP4 39
 
 /* matrix slots of a MoE layer */
 #define DNB_MAT_GATE 0
@@ -87,6 +93,7 @@ uint64_t dnb_launch_count(dnb_ctx* ctx);
  *   24       expert-parallel decode: a peer's result rows did not arrive
  *   23       grid barrier of the fused one-token kernel
  *   25       the tensor-core router GEMM of a prefill chunk (stage or accumulator barrier)
+ *   27-29    a dense product (microscaled 4-bit or 16-bit): stage, accumulator or drain barrier
  *   26       no wait: a grouped kernel (mma.sync or tcgen05) found its shared memory to start elsewhere than the context has it
  * What the reference promises for a GPU call that did not complete -- "false: out
  * untouched, the caller recomputes" (cuda.rs:21024-21027, 8785-8788) -- holds here too:
@@ -170,6 +177,59 @@ int dnb_set_q4k_int(dnb_ctx* ctx, int on);
  * two differ by summation order only; an A/B knob.  (dnb_router_topk_static always runs the fp32 kernel: where
  * the tcgen05 kernel would take the call its weights agree within rounding, not bit for bit.) */
 int dnb_set_router_tc(dnb_ctx* ctx, int on);
+
+/* ---- microscaled 4-bit matrices ---------------------------------------------------
+ * No counterpart in the reference, whose 4-bit formats are integers that are decoded before they are multiplied; the
+ * tensor cores multiply this one as it is.  An element is a 4-bit floating point number (sign, two exponent bits, one
+ * mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), 32 of a row share a power of two.  A matrix [rows][k], k a multiple of 32,
+ * is two arrays in device memory, both starting at a multiple of 16 bytes:
+ *   codes  [rows][k / 2]: element 2 i of a row in the low half of its byte i;
+ *   scales: a byte for each 32 elements, standing for 2^(byte - 127), or NaN where it is 255, in tiles of 128 rows x 4
+ *     scales: scale j of row r at byte ((r / 128) * ceil(k / 128) + j / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + j % 4.
+ *     Of a tile that reaches beyond the matrix, scales past a row's end are zero; rows past the last are never looked at.
+ * All pointers are device pointers of the context's device; the calls are asynchronous on the context's stream, allocate
+ * nothing and keep nothing, so that they can be captured into a graph.  Results must not overlap operands.  No tokens
+ * (rows, nt = 0) is DNB_OK and does nothing.  DNB_DECLINED: a type, k or alignment that the kernels do not take.
+ *   dnb_mx4_bytes: how long the two arrays are.
+ *   dnb_mx4_quantize_dev: rows of F32, F16 or BF16, ldx elements apart (aligned as their type), to such a matrix.  The scale's
+ *       exponent is floor(log2(largest magnitude of the 32)) - 2, at least -127; elements are rounded to nearest, ties to
+ *       even, and to 6 beyond it.  32 elements with an infinity or a NaN among them get scale 255 and codes of zero.
+ *       Type MXFP4: rows of a GGUF file's 17-byte blocks, laid out anew (weights: once, as they are loaded); ldx a multiple of 32.
+ *   dnb_mx4_dequantize_dev: back to F32 or BF16 (exact, but for overflow) or F16 (rounded), rows ldo elements apart.
+ *   dnb_mx4_gemm_dev: out[t][r] = sum_i X[t][i] W[r][i] for nt rows X and n rows W, out F32, F16 or BF16.  Products are exact, sums 32 bits.
+ *   dnb_mx4_gated_dev: out[t][r] = act(g) * u with g = sum_i X[t][i] G[r][i], u = sum_i X[t][i] U[r][i] (cf. dnb_moe_experts); out as
+ *       before, or MXFP4 with n a multiple of 32: quantised as above into out (codes) and out_scales, the operand of the next product.
+ * The same inputs give the same bits on every run; a row's bits may depend on how many rows the call has (the sum over k is
+ * divided among thread blocks where there are few). */
+#define DNB_ACT_SILU 0  /* v / (1 + exp(-v)) */
+#define DNB_ACT_GELU 1  /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
+int dnb_mx4_bytes(int rows, int k, size_t* codes, size_t* scales);
+int dnb_mx4_quantize_dev(dnb_ctx* ctx, int type, const void* x_dev, size_t ldx, int rows, int k, void* codes_dev, void* scales_dev);
+int dnb_mx4_dequantize_dev(dnb_ctx* ctx, const void* codes_dev, const void* scales_dev, int rows, int k, int type, void* out_dev,
+                           size_t ldo);
+int dnb_mx4_gemm_dev(dnb_ctx* ctx, const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, int nt, int k,
+                     int n, int type, void* out_dev, size_t ldo);
+int dnb_mx4_gated_dev(dnb_ctx* ctx, int act, const void* x_codes, const void* x_scales, const void* gate_codes, const void* gate_scales,
+                      const void* up_codes, const void* up_scales, int nt, int k, int n, int type, void* out_dev, void* out_scales_dev,
+                      size_t ldo);
+
+/* ---- gated feed-forward block on 16-bit operands ---------------------------------------
+ * Both projections, the activation and the product of a dense feed-forward block (the reference's expert form:
+ * moe_expert.rs silu(gate x) * up x) and its gradients.  type: F16 or BF16, of all operands and results but pre (fp32).
+ * x [nt][k], gate and up [n][k]; k and n multiples of 8; rows of x, dout ldx, ldd (multiples of 8) elements apart, of out and
+ * dx ldo, lddx; operands and pre, dpre start at multiples of 16 bytes.  Device pointers, asynchronous, nothing allocated, as above.
+ *   dnb_gated_dev: g = x gate^T, u = x up^T, out = act(g) * u.  pre (NULL without a backward pass): [2][nt][n], g and then u.
+ *   dnb_gated_backward_dev: from pre and dout [nt][n], the gradient of out:
+ *       dpre [2][nt][n]: dout * u * act'(g) and dout * act(g), rounded to the type (wanted in any case: the operands of the rest),
+ *       dx [nt][k] = dpre[0] gate + dpre[1] up, or NULL (x is not looked at without the weights' gradients, nor gate and up without dx),
+ *       dgate, dup [n][k] = dpre[0]^T x, dpre[1]^T x, or both NULL.  With nt = 0 they are zeros.
+ * 4-bit weights have no gradient of their own; dx for them: dnb_mx4_dequantize_dev to BF16 is exact.
+ * A row's bits may depend on nt, as above. */
+int dnb_gated_dev(dnb_ctx* ctx, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev, int nt, int k,
+                  int n, void* out_dev, size_t ldo, float* pre_dev);
+int dnb_gated_backward_dev(dnb_ctx* ctx, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev,
+                           const float* pre_dev, const void* dout_dev, size_t ldd, int nt, int k, int n, void* dpre_dev, void* dx_dev,
+                           size_t lddx, void* dgate_dev, void* dup_dev);
 
 /* ---- MoE model: resident expert table ----------------------------------------
  * Replaces the VRAM/RAM/SSD expert tiers (expert_vram.rs:1-60; use at
