@@ -1,0 +1,433 @@
+// Dense products of many rows on tcgen05, two SMs a tile (cta_group::2): D[m][n] = sum_k A[m][k] B[n][k], out[m][n] with n contiguous.
+//
+// Tiles of 256 x 256: each CTA of a pair holds 128 rows of A and 128 of B, the MMA (M 256, N 256) reads B from both, and a CTA's
+// tensor memory gets its 128 rows of D: half the operand bytes of two separate 128 x 256 tiles, through L2 as well as into the MMAs.
+// Gated: the B tile is 128 rows of gate in one CTA and the same 128 of up in the other, so that a thread that reads a row of D has g and u
+// of the same features: 256 x 128 results from one MMA.
+// Operands as in dense_tc.cuh: 4 bits with scales in tensor memory, or 16 bits with rows along K or along m / n.
+//
+// A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight
+// warps read the accumulators: a thread a row, 32 columns at a time, through 4 KB of shared memory a warp and out by TMA stores (or, where
+// rows do not start at multiples of 16 bytes, in whole rows by plain stores).  16 bits: two accumulators; 4 bits, where the scales take the
+// room: one, drained to registers at once so that the next tile's MMAs need not wait for the stores.
+#pragma once
+#include "dense_tc.cuh"
+
+namespace dnb {
+namespace dp {
+using namespace dt;
+
+struct Params {
+    CUtensorMap a[2], b[2];         // operands
+    CUtensorMap sa, sb[2];          // scale tiles, 512 bytes a row (4 bit)
+    CUtensorMap out[2], pre[2];     // results
+    int M, N, K;                    // N: columns of the output
+    int passes;                     // 2: the sum goes on over a[1], b[1]
+    int both;                       // 2: twice the tiles, the second half with a[1] to the second output
+    int tiles_m, tiles_n;
+    int idesc_type, out_type, act;
+    bool tma_out, keep;             // keep: g and u to pre
+    void* outp[2];
+    uint8_t* out_scales;
+    size_t ldo;
+    int* status;
+};
+
+template <bool FP4_, bool GATED_, bool AMN_ = false, bool BMN_ = false>
+struct Cfg {
+    static constexpr bool FP4 = FP4_, GATED = GATED_, AMN = AMN_, BMN = BMN_;
+    static constexpr int BK = FP4 ? 256 : 64;
+    static constexpr int HALF = 128 * 128;                     // a CTA's half of an operand's tile
+    static constexpr int SF = FP4 ? 3 * 1024 : 0;              // scales: 128 rows of A, 256 of B, 256 of K
+    static constexpr int STAGE = 2 * HALF + SF;
+    static constexpr int STAGES = FP4 ? 5 : 6;
+    static constexpr int STAGING = EPI_WARPS * 4096;
+    static constexpr int ACC = 256, BUFS = FP4 ? 1 : 2;
+    static constexpr int SF_COLS = 24;                         // 8 of A, 16 of B
+    static constexpr int COLS = 512;
+    static constexpr int NOUT = GATED ? 128 : 256;             // columns of the output a tile
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE + STAGING + 1024 + 256;
+};
+
+// ---- PTX of pairs ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(s32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {  // the barrier of both CTAs
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void pair_mma16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_mma4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void pair_scales(uint32_t taddr, uint32_t smem) {  // each CTA's own 512 bytes to its own tensor memory
+    const uint64_t desc = ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | ((smem >> 4) & 0x3FFFu);
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void pair_alloc(uint32_t* slot) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s32(slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_free(uint32_t base) { asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory"); }
+// 32 columns of this thread's row.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+// ---- results ----------------------------------------------------------------------------------------------------------------------
+template <int OUT>
+__device__ __forceinline__ uint32_t two(float a, float b) {
+    if constexpr (OUT == T_F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// 32 rows x 32 columns of a warp, a row a lane, from (row0, col0) of a [M][N] matrix.  buf: the warp's 4 KB; rows of 64 or 128 bytes in the
+// swizzle of the tensor map, which keeps the 16-byte stores of eight lanes apart.
+template <int OUT>
+__device__ __forceinline__ void chunk_out(const CUtensorMap* map, bool tma, void* out, size_t ldo, int M, int N, int row0, int col0, const float (&v)[32], uint8_t* buf,
+                                          int lane) {
+    if (row0 >= M || col0 >= N) return;  // the whole warp
+    if (tma) {
+        if (lane == 0) store_read();
+    }
+    __syncwarp();
+    if constexpr (OUT == T_F32) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(two<OUT>(v[8 * c], v[8 * c + 1]), two<OUT>(v[8 * c + 2], v[8 * c + 3]), two<OUT>(v[8 * c + 4], v[8 * c + 5]), two<OUT>(v[8 * c + 6], v[8 * c + 7]));
+    }
+    if (tma) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) store_2d(map, col0, row0, s32(buf));
+    } else {
+        __syncwarp();
+        if (col0 + lane < N) {
+            const int rows = min(32, M - row0);
+            for (int r = 0; r < rows; ++r) {
+                const size_t at = (size_t)(row0 + r) * ldo + col0 + lane;
+                if constexpr (OUT == T_F32)
+                    reinterpret_cast<float*>(out)[at] = *reinterpret_cast<const float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                else
+                    reinterpret_cast<uint16_t*>(out)[at] = *reinterpret_cast<const uint16_t*>(buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+            }
+        }
+        __syncwarp();
+    }
+}
+// 32 features of a row as one 4-bit block.
+__device__ __forceinline__ void block_out(const Params& p, int row, int col, const float (&v)[32]) {
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+    const uint32_t e = scale_byte(mx);
+    const float by = scale_inverse(e);
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float w[8] = {v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3], v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]};
+        c[i] = e == 255 ? 0u : e2m1_eight(w, by);
+    }
+    if (row >= p.M) return;
+    if (col < p.N) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.outp[0]) + ((size_t)row * p.N + col) / 2) = make_uint4(c[0], c[1], c[2], c[3]);
+    p.out_scales[scale_at(row, col >> 5, (p.N + 127) >> 7)] = (uint8_t)(col < p.N ? e : 0u);
+}
+
+template <class C, int OUT>
+__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t* buf, int lane, uint32_t drained) {
+    // This thread's columns: 32 at a time; gated: 32 of gate and of up.
+    constexpr int CHUNKS = C::GATED ? 2 : 4;
+    constexpr bool DRAIN = C::BUFS == 1;
+    float v[DRAIN ? 4 : C::GATED ? 2 : 1][32];
+    const int at = half * (C::GATED ? 64 : 128);
+    if constexpr (DRAIN) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            tmem_ld32(ta + at + 32 * c, v[c]);
+            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, v[2 + c]);
+        }
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) remote_arrive(drained);
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int g = DRAIN ? c : 0, u = DRAIN ? 2 + c : C::GATED ? 1 : 0, col = n0 + at + 32 * c;
+        if constexpr (!DRAIN) {
+            tmem_ld32(ta + at + 32 * c, v[0]);
+            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, v[1]);
+            tmem_ld_wait();
+        }
+        if constexpr (C::GATED) {
+            if (p.keep) {
+                chunk_out<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, v[g], buf, lane);
+                chunk_out<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, v[u], buf, lane);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[g][j] = act_of(p.act, v[g][j]) * v[u][j];
+        }
+        if constexpr (OUT == T_MXFP4) block_out(p, row0 + lane, col, v[g]);
+        else chunk_out<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col, v[g], buf, lane);
+    }
+    if constexpr (!DRAIN) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) remote_arrive(drained);
+    }
+}
+
+__device__ __forceinline__ void pair_tile(const Params& p, int t, int& m, int& n, int& which) {
+    constexpr int G = 8;  // 8 x 256 rows of A by about as many of B are in flight
+    const int per = p.tiles_m * p.tiles_n;
+    which = t >= per;
+    if (which) t -= per;
+    const int g = t / (G * p.tiles_n), in = t - g * G * p.tiles_n, rows = min(G, p.tiles_m - g * G);
+    m = g * G + in % rows;
+    n = in / rows;
+}
+
+template <class C>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_kernel(const __grid_constant__ Params p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* staging = smem + C::STAGES * C::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* tfull = empty + C::STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    if (tid == 0) {
+        for (int i = 0; i < C::STAGES; ++i) {
+            mb_init(&full[i], 1);   // the leader's: its own expect_tx; bytes of both CTAs
+            mb_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mb_init(&tfull[i], 1);
+            mb_init(&tempty[i], 2 * EPI_WARPS);  // the leader's: both CTAs' warps
+        }
+        fence_mbarrier_init();
+    }
+    if (warp == 1) pair_alloc(tmem_slot);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const int kch = (p.K + C::BK - 1) / C::BK, chunks = kch * p.passes, tiles = p.tiles_m * p.tiles_n * p.both;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    bool ok = true;
+    int m, n, which;
+
+    if (warp == 0) {
+        // ---------------- TMA ----------------
+        const int nkb = (p.K + 127) >> 7;
+        int it = 0;
+        for (int t = first; t < tiles && ok; t += step) {
+            pair_tile(p, t, m, n, which);
+            const int m0 = m * 256 + (int)rank * 128, n0 = C::GATED ? n * 128 : n * 256 + (int)rank * 128;
+            for (int c = 0; c < chunks; ++c, ++it) {
+                const int st = it % C::STAGES, use = it / C::STAGES;
+                if (use > 0) ok = warp_all(mb_wait(&empty[st], (uint32_t)(use - 1) & 1u, p.status, kWaitStage));
+                if (!ok) break;
+                if (elect_one()) {
+                    uint8_t *sa = smem + st * C::STAGE, *sb = sa + C::HALF;
+                    const int pass = c >= kch, kc = pass ? c - kch : c;
+                    const uint32_t bar = in_cta(s32(&full[st]), 0);
+                    if (rank == 0) mb_expect_tx(&full[st], 2u * C::STAGE);
+                    const CUtensorMap *ma = &p.a[pass | which], *mb = &p.b[C::GATED ? (int)rank : pass];
+                    if constexpr (C::AMN) {
+                        pair_load_2d(sa, ma, m0, kc * 64, bar);
+                        pair_load_2d(sa + 8192, ma, m0 + 64, kc * 64, bar);
+                    } else {
+                        pair_load_2d(sa, ma, kc * (C::FP4 ? 128 : 64), m0, bar);
+                    }
+                    if constexpr (C::BMN) {
+                        pair_load_2d(sb, mb, n0, kc * 64, bar);
+                        pair_load_2d(sb + 8192, mb, n0 + 64, kc * 64, bar);
+                    } else {
+                        pair_load_2d(sb, mb, kc * (C::FP4 ? 128 : 64), n0, bar);
+                    }
+                    if constexpr (C::FP4) {
+                        uint8_t* sf = sb + C::HALF;
+                        pair_load_2d(sf, &p.sa, 0, (m0 >> 7) * nkb + 2 * kc, bar);
+                        pair_load_2d(sf + 1024, &p.sb[0], 0, (C::GATED ? n : 2 * n) * nkb + 2 * kc, bar);
+                        pair_load_2d(sf + 2048, &p.sb[C::GATED], 0, (C::GATED ? n : 2 * n + 1) * nkb + 2 * kc, bar);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok && rank == 0)  // copies in flight, of both CTAs, end before their shared memory is given up
+            for (int i = max(0, it - C::STAGES); i < it; ++i) mb_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
+    } else if (warp == 1) {
+        // ---------------- MMA issue: the leader's thread for both ----------------
+        if (rank == 0) {
+            const uint32_t smem_lo = (s32(smem) & 0x3FFFFu) >> 4;  // in a cluster an address has its CTA's rank above
+            constexpr uint32_t LA = (C::AMN ? (8192u >> 4) : 1u) << 16, LB = (C::BMN ? (8192u >> 4) : 1u) << 16;
+            constexpr uint32_t KA = C::AMN ? 128 : 2, KB = C::BMN ? 128 : 2;
+            const uint32_t sf_tmem = tmem + C::BUFS * C::ACC;
+            const uint32_t idesc = C::FP4 ? (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | (1u << 23) | ((256u >> 7) << 27)
+                                          : (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) |
+                                                ((uint32_t)C::BMN << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+            int it = 0, nt = 0;
+            for (int t = first; t < tiles && ok; t += step, ++nt) {
+                const int buf = nt % C::BUFS, use = nt / C::BUFS;
+                if (use > 0) ok = warp_all(mb_wait(&tempty[buf], (uint32_t)(use - 1) & 1u, p.status, kWaitDrain));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + buf * C::ACC;
+                for (int c = 0; c < chunks; ++c, ++it) {
+                    const int st = it % C::STAGES;
+                    ok = warp_all(mb_wait(&full[st], (uint32_t)(it / C::STAGES) & 1u, p.status, kWaitStage));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t a0 = smem_lo + (uint32_t)(st * (C::STAGE >> 4)), b0 = a0 + (C::HALF >> 4);
+                        if constexpr (C::FP4) {
+                            const uint32_t sf = b0 + (C::HALF >> 4), ts = sf_tmem + (it & 1) * C::SF_COLS;
+                            const int left = p.K - c * C::BK, kbs = left > 128 ? 2 : 1, steps = left >= C::BK ? 4 : (left + 63) >> 6;
+                            for (int kb = 0; kb < kbs; ++kb) {
+                                pair_scales(ts + kb * 4, (sf + kb * 32) << 4);
+                                pair_scales(ts + 8 + kb * 8, (sf + 64 + kb * 32) << 4);
+                                pair_scales(ts + 12 + kb * 8, (sf + 128 + kb * 32) << 4);
+                            }
+                            for (int ks = 0; ks < steps; ++ks)
+                                pair_mma4(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc | ((uint32_t)(ks & 1) << 30) | ((uint32_t)(ks & 1) << 5),
+                                          ts + (ks >> 1) * 4, ts + 8 + (ks >> 1) * 8, c > 0 || ks > 0);
+                        } else {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks)
+                                pair_mma16(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc, c > 0 || ks > 0);
+                        }
+                        pair_commit(&empty[st]);
+                        if (c == chunks - 1) pair_commit(&tfull[buf]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        // ---------------- results ----------------
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        uint8_t* buf_s = staging + (warp - 2) * 4096;
+        int nt = 0;
+        for (int t = first; t < tiles && ok; t += step, ++nt) {
+            const int buf = nt % C::BUFS, use = nt / C::BUFS;
+            ok = warp_all(mb_wait(&tfull[buf], (uint32_t)use & 1u, p.status, kWaitAcc));
+            if (!ok) break;
+            tc_fence_after();
+            pair_tile(p, t, m, n, which);
+            const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
+            const uint32_t ta = tmem + buf * C::ACC + ((uint32_t)(quad * 32) << 16), drained = in_cta(s32(&tempty[buf]), 0);
+            switch (p.out_type) {
+                case T_F16: results<C, T_F16>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
+                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
+                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
+                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, ta, buf_s, lane, drained);
+            }
+        }
+        if (lane == 0) store_done();
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // nobody's shared or tensor memory goes while the other may still use it
+    if (warp == 1) {
+        tc_fence_after();
+        pair_free(tmem);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------------
+// Scale tiles of `rows` rows, as a matrix of 512-byte rows; boxes of two.
+inline int scale_map(CUtensorMap* m, const void* scales, uint64_t rows, uint64_t k) {
+    return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, scales, (rows + 127) / 128 * ((k + 127) / 128), 128, 512, 2, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+// Results [rows][cols] of `type`, in the epilogue's chunks.
+inline int result_map(CUtensorMap* m, int type, const void* out, uint64_t rows, uint64_t cols, uint64_t ld) {
+    const bool f32 = type == T_F32;
+    return tiled_map(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, f32 ? 4 : 2, out, rows,
+                     cols, ld * (f32 ? 4 : 2), 32, 32, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// p: M, N, K, passes, both, type, act, outp, out_scales, ldo; maps of scales and pre where there are any.
+template <class C>
+int launch_pair(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* b, int nb, int type, const char* name) {
+    int rc;
+    for (int i = 0; i < na; ++i)
+        if ((rc = operand_map<C::FP4>(&p.a[i], a[i], C::AMN ? 64 : 128, type))) return rc;
+    for (int i = 0; i < nb; ++i)
+        if ((rc = operand_map<C::FP4>(&p.b[i], b[i], C::BMN ? 64 : 128, type))) return rc;
+    const int es = p.out_type == T_F32 ? 4 : 2;
+    // Rows that end inside 16 bytes would be written to their end.
+    p.tma_out = p.out_type != T_MXFP4 && p.ldo * es % 16 == 0 && (size_t)p.N * es % 16 == 0;
+    for (int i = 0; i < p.both; ++i) p.tma_out = p.tma_out && ((uintptr_t)p.outp[i] & 15) == 0;
+    if (p.tma_out)
+        for (int i = 0; i < p.both; ++i)
+            if ((rc = result_map(&p.out[i], p.out_type, p.outp[i], p.M, p.N, p.ldo))) return rc;
+    p.idesc_type = type == T_BF16;
+    p.status = c->status;
+    p.tiles_m = (p.M + 255) / 256;
+    p.tiles_n = (p.N + C::NOUT - 1) / C::NOUT;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.both;
+    if (tiles > 0x3fffffff) {
+        set_error("%s: %d x %d results are more than one launch takes", name, p.M, p.N);
+        return DNB_DECLINED;
+    }
+    const int pairs = c->sm_count / 2;
+    static SmemGrant grant;
+    DNB_CUDA(grant_smem(grant, c->device, pair_kernel<C>, C::SMEM));
+    ProfScope prof_(c, c->stream, name);
+    DNB_CUDA(launch_k(pair_kernel<C>, dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), dim3(NTHREADS), C::SMEM, c->stream, c->use_pdl, p));
+    c->launches++;
+    return DNB_OK;
+}
+
+}  // namespace dp
+}  // namespace dnb

@@ -1,15 +1,14 @@
-// Dense products on tcgen05: D[m][n] = sum_k A[m][k] B[n][k], stored as out[n][m] (m contiguous), for
+// Dense products of few rows (up to 128) on tcgen05: D[m][n] = sum_k A[m][k] B[n][k], stored as out[n][m] (m contiguous), for
 //   * 4-bit microscaled operands (kind::mxf4, 2^x scales of 32 elements taken from tensor memory) and 16-bit ones (kind::f16),
-//   * operands whose rows run along K, or (16 bit) along m or n, so that no gradient needs a transposed copy,
+//   * weights A whose rows run along K, or (16 bit) along m, so that dx needs no transposed copy,
 //   * one A, or two with an accumulator each (gate and up) that the epilogue joins: act(g) * u.
 // m is the feature that is contiguous in the output: lane l of TMEM row quarter q holds m = 32 q + l, so that the stores of a column
 // are whole 64- or 128-byte lines without a trip through shared memory, a block of 32 features is one warp's column (the epilogue
-// can quantise), and few tokens make narrow tiles (n from 16) under full-height ones of weights.
+// can quantise), and few tokens make narrow tiles (n from 16) under full-height ones of weights, whose bytes are what such a product costs.
 //
 // One CTA: warp 0 moves tiles by TMA through a ring of stages of 128 bytes of K a row, warp 1 issues the MMAs, eight warps read the
-// accumulators (two a row quarter).  Large outputs: one CTA per SM walks tiles, accumulators twice where TMEM has room, so that the
-// epilogue of a tile runs under the next one's MMAs.  Small outputs: a cluster splits K and its CTAs' partial sums are added through
-// distributed shared memory in ascending rank order (no workspace, no atomics: the same bits on every run).
+// accumulators (two a row quarter).  Few results: a cluster splits K and its CTAs' partial sums are added through distributed shared
+// memory in ascending rank order (no workspace, no atomics: the same bits on every run).
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -30,16 +29,15 @@ constexpr int kWaitStage = 27, kWaitAcc = 28, kWaitDrain = 29;  // status codes 
 enum Act { ACT_NONE = -1, ACT_SILU = 0, ACT_GELU = 1 };
 
 struct Params {
-    CUtensorMap a[2], b[2];
+    CUtensorMap a[2], b[2];         // b[1]: of the second pass
     const uint8_t* sa[2];           // scale tiles of A (4 bit)
     const uint8_t* sb;              // and of B
     int M, N, K;
     int passes;                     // 2: the sum goes on over a[1], b[1]
-    int both;                       // 2: twice the tiles, the second half with b[1] to out[1]
-    int tiles_m, tiles_n, splits;
+    int splits;
     int idesc_type;                 // 16 bit: 0 fp16, 1 bf16
     int out_type, act;
-    void* out[2];
+    void* out;
     uint8_t* out_scales;            // MXFP4 results
     float* pre;                     // gate and up before the activation [2][N][M], or null
     size_t ldo;                     // elements between rows of out
@@ -48,27 +46,25 @@ struct Params {
 
 constexpr int pow2_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
 
-template <bool FP4_, int NA_, int BN_, bool AMN_ = false, bool BMN_ = false>
+template <bool FP4_, int NA_, int BN_, bool AMN_ = false>
 struct Cfg {
-    static constexpr bool FP4 = FP4_, AMN = AMN_, BMN = BMN_;
+    static constexpr bool FP4 = FP4_, AMN = AMN_;
     static constexpr int NA = NA_, BN = BN_;
     static constexpr int BK = FP4 ? 256 : 64;               // 128 bytes of a row
     static constexpr int A_BYTES = TM * 128, B_BYTES = BN * 128;
     static constexpr int SFA = FP4 ? 1024 : 0;              // scales of 128 rows x 256 elements
-    static constexpr int SFB_TILES = BN > 128 ? 2 : 1;
-    static constexpr int SFB = FP4 ? SFB_TILES * 1024 : 0;
-    static constexpr int STAGE = NA * A_BYTES + B_BYTES + NA * SFA + SFB;
+    static constexpr int STAGE = NA * A_BYTES + B_BYTES + (NA + 1) * SFA;
     static constexpr int PER_SM = BN < 128 ? 2 : 1;
     static constexpr int BUDGET = PER_SM == 2 ? 115712 - 1536 : 232448 - 1536;
     static constexpr int FIT = BUDGET / STAGE;
     static constexpr int STAGES = FIT > 8 ? 8 : FIT;
     static constexpr int ACC = NA * BN;
-    static constexpr int SF_COLS = FP4 ? NA * 8 + SFB_TILES * 8 : 0;   // one of two buffers
+    static constexpr int SF_COLS = FP4 ? NA * 8 + 8 : 0;   // one of two buffers
     static constexpr int BUFS = BN >= 128 && 2 * ACC + 2 * SF_COLS <= 512 ? 2 : 1;
     static constexpr int COLS = pow2_cols(BUFS * ACC + 2 * SF_COLS);
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 512;
     static_assert(STAGES >= 2 && PER_SM * COLS <= 512, "no room");
-    static_assert(!FP4 || (!AMN && !BMN), "4-bit operands lie along K");
+    static_assert(!FP4 || !AMN, "4-bit operands lie along K");
 };
 
 __device__ __forceinline__ float act_of(int act, float g) {
@@ -140,24 +136,9 @@ __device__ __forceinline__ float peer_float(uint32_t smem, uint32_t rank) {
     return v;
 }
 
-struct Tile { int m, n, which; };
-template <class C>
-__device__ __forceinline__ Tile tile_of(const Params& p, int t) {
-    // Groups of 16 (8 with two A) rows of tiles, column by column: the tiles in flight read about as much of A as of B, and little of both.
-    constexpr int G = C::NA == 2 ? 8 : 16;
-    const int per = p.tiles_m * p.tiles_n;
-    Tile r;
-    r.which = t >= per;
-    if (r.which) t -= per;
-    const int g = t / (G * p.tiles_n), in = t - g * G * p.tiles_n, rows = min(G, p.tiles_m - g * G);
-    r.m = g * G + in % rows;
-    r.n = in / rows;
-    return r;
-}
-
 // One column of results: feature m of this lane (beyond M: nothing stored), row n of the output.
 template <class C, int OUT>
-__device__ __forceinline__ void emit(const Params& p, int which, int m, int n, float v0, float v1) {
+__device__ __forceinline__ void emit(const Params& p, int m, int n, float v0, float v1) {
     float v = v0;
     if constexpr (C::NA == 2) {
         v = act_of(p.act, v0) * v1;
@@ -176,16 +157,16 @@ __device__ __forceinline__ void emit(const Params& p, int which, int m, int n, f
         c <<= 8 * ((lane >> 1) & 3);
         c |= __shfl_xor_sync(0xffffffffu, c, 2);
         c |= __shfl_xor_sync(0xffffffffu, c, 4);
-        if (m < p.M && (lane & 7) == 0) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out[0]) + ((size_t)n * p.M + m) / 2) = c;
+        if (m < p.M && (lane & 7) == 0) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + ((size_t)n * p.M + m) / 2) = c;
         if (lane == 0) p.out_scales[scale_at(n, m >> 5, (p.M + 127) >> 7)] = (uint8_t)(m < p.M ? e : 0u);
     } else {
-        if (m < p.M) put<OUT>(p.out[which], (size_t)n * p.ldo + m, v);
+        if (m < p.M) put<OUT>(p.out, (size_t)n * p.ldo + m, v);
     }
 }
 
 template <class C, int OUT>
-__device__ __forceinline__ void tile_out(const Params& p, const Tile& t, uint32_t tacc, int quad, int half, int lane) {
-    const int m = t.m * TM + quad * 32 + lane, n0 = t.n * C::BN;
+__device__ __forceinline__ void tile_out(const Params& p, int tile, uint32_t tacc, int quad, int half, int lane) {
+    const int m = tile * TM + quad * 32 + lane;
     const uint32_t ta = tacc + ((uint32_t)(quad * 32) << 16);
 #pragma unroll 1
     for (int g = half; g < C::BN / 16; g += 2) {
@@ -195,22 +176,22 @@ __device__ __forceinline__ void tile_out(const Params& p, const Tile& t, uint32_
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int n = n0 + 16 * g + j;
-            if (n < p.N) emit<C, OUT>(p, t.which, m, n, __uint_as_float(v0[j]), C::NA == 2 ? __uint_as_float(v1[j]) : 0.f);
+            const int n = 16 * g + j;
+            if (n < p.N) emit<C, OUT>(p, m, n, __uint_as_float(v0[j]), C::NA == 2 ? __uint_as_float(v1[j]) : 0.f);
         }
     }
 }
 
 template <class C, int OUT>
-__device__ __forceinline__ void split_out(const Params& p, const Tile& t, uint32_t red, uint32_t rank, int quad, int half, int lane) {
-    const int m = t.m * TM + quad * 32 + lane, n0 = t.n * C::BN;
-    for (int c = (int)rank + p.splits * half; c < C::BN && n0 + c < p.N; c += 2 * p.splits) {
+__device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t red, uint32_t rank, int quad, int half, int lane) {
+    const int m = tile * TM + quad * 32 + lane;
+    for (int c = (int)rank + p.splits * half; c < p.N; c += 2 * p.splits) {
         float s0 = 0.f, s1 = 0.f;
         for (int r = 0; r < p.splits; ++r) {
             s0 += peer_float(red + 4u * (uint32_t)(c * TM + quad * 32 + lane), r);
             if constexpr (C::NA == 2) s1 += peer_float(red + 4u * (uint32_t)((C::BN + c) * TM + quad * 32 + lane), r);
         }
-        emit<C, OUT>(p, t.which, m, n0 + c, s0, s1);
+        emit<C, OUT>(p, m, c, s0, s1);
     }
 }
 
@@ -247,7 +228,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
     const int kch = (p.K + C::BK - 1) / C::BK, chunks = kch * p.passes;
     const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
     const int c0 = (int)((long long)chunks * rank / p.splits), c1 = (int)((long long)chunks * (rank + 1) / p.splits);
-    const int tiles = p.tiles_m * p.tiles_n * p.both;
+    const int tiles = (p.M + TM - 1) / TM;
     const int first = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, step = p.splits > 1 ? tiles : gridDim.x;
     const int nkb = (p.K + 127) >> 7;  // scale tiles along K
     bool ok = true;
@@ -256,8 +237,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
         // ---------------- TMA ----------------
         int it = 0;
         for (int t = first; t < tiles && ok; t += step) {
-            const Tile tl = tile_of<C>(p, t);
-            const int m0 = tl.m * TM, n0 = tl.n * C::BN;
+            const int m0 = t * TM;
             for (int c = c0; c < c1; ++c, ++it) {
                 const int st = it % C::STAGES, n = it / C::STAGES;
                 if (n > 0) ok = warp_all(mb_wait(&empty[st], (uint32_t)(n - 1) & 1u, p.status, kWaitStage));
@@ -265,12 +245,8 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
                 if (elect_one()) {
                     uint8_t* s = smem + st * C::STAGE;
                     const int pass = c >= kch, kc = pass ? c - kch : c;
-                    int kbs = 0, bt = 0;
-                    if constexpr (C::FP4) {
-                        kbs = min(2, nkb - 2 * kc);
-                        bt = min(C::SFB_TILES, ((p.N + 127) >> 7) - (n0 >> 7));
-                    }
-                    mb_expect_tx(&full[st], (uint32_t)(C::NA * C::A_BYTES + C::B_BYTES + (C::NA + bt) * kbs * 512));
+                    const int kbs = C::FP4 ? min(2, nkb - 2 * kc) : 0;
+                    mb_expect_tx(&full[st], (uint32_t)(C::NA * C::A_BYTES + C::B_BYTES + (C::NA + 1) * kbs * 512));
 #pragma unroll
                     for (int a = 0; a < C::NA; ++a) {
                         const CUtensorMap* map = &p.a[C::NA == 2 ? a : pass];
@@ -282,19 +258,12 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
                         }
                     }
                     uint8_t* sb = s + C::NA * C::A_BYTES;
-                    const CUtensorMap* map = &p.b[pass | tl.which];
-                    if constexpr (C::BMN) {
-#pragma unroll
-                        for (int i = 0; i < C::BN / 64; ++i) tma_load_2d(sb + i * 8192, map, n0 + 64 * i, kc * 64, &full[st]);
-                    } else {
-                        tma_load_2d(sb, map, kc * (C::FP4 ? 128 : 64), n0, &full[st]);
-                    }
+                    tma_load_2d(sb, &p.b[pass], kc * (C::FP4 ? 128 : 64), 0, &full[st]);
                     if constexpr (C::FP4) {
                         uint8_t* sf = sb + C::B_BYTES;
                         for (int a = 0; a < C::NA; ++a)
-                            bulk_load(sf + a * 1024, p.sa[a] + ((size_t)tl.m * nkb + 2 * kc) * 512, kbs * 512, &full[st]);
-                        for (int i = 0; i < bt; ++i)
-                            bulk_load(sf + (C::NA + i) * 1024, p.sb + ((size_t)((n0 >> 7) + i) * nkb + 2 * kc) * 512, kbs * 512, &full[st]);
+                            bulk_load(sf + a * 1024, p.sa[a] + ((size_t)t * nkb + 2 * kc) * 512, kbs * 512, &full[st]);
+                        bulk_load(sf + C::NA * 1024, p.sb + (size_t)2 * kc * 512, kbs * 512, &full[st]);
                     }
                 }
                 __syncwarp();
@@ -304,16 +273,16 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
             for (int i = max(0, it - C::STAGES); i < it; ++i) mb_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
     } else if (warp == 1) {
         // ---------------- MMA issue ----------------
-        const uint32_t smem_lo = s32(smem) >> 4;
-        constexpr uint32_t LA = (C::AMN ? (8192u >> 4) : 1u) << 16, LB = (C::BMN ? (8192u >> 4) : 1u) << 16;
-        constexpr uint32_t KA = C::AMN ? 128 : 2, KB = C::BMN ? 128 : 2;  // bytes / 16 from one K step of an MMA to the next
+        const uint32_t smem_lo = (s32(smem) & 0x3FFFFu) >> 4;  // in a cluster an address has its CTA's rank above
+        constexpr uint32_t LA = (C::AMN ? (8192u >> 4) : 1u) << 16, LB = 1u << 16;
+        constexpr uint32_t KA = C::AMN ? 128 : 2, KB = 2;  // bytes / 16 from one K step of an MMA to the next
         const uint32_t sf_tmem = tmem + C::BUFS * C::ACC;
         uint32_t idesc;
         if constexpr (C::FP4)  // e2m1 operands, 2^x scales
             idesc = (1u << 7) | (1u << 10) | ((uint32_t)(C::BN >> 3) << 17) | (1u << 23) | (1u << 27);
         else
-            idesc = (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) | ((uint32_t)C::BMN << 16) |
-                    ((uint32_t)(C::BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+            idesc = (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) | ((uint32_t)(C::BN >> 3) << 17) |
+                    ((uint32_t)(TM >> 4) << 24);
         int it = 0, nt = 0;
         for (int t = first; t < tiles && ok; t += step, ++nt) {
             const int buf = nt % C::BUFS, use = nt / C::BUFS;
@@ -321,7 +290,6 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
             if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem + buf * C::ACC;
-            const int n_sf = C::FP4 ? ((tile_of<C>(p, t).n * C::BN) & 127) >> 5 : 0;  // narrow tiles start inside a tile of scales
             for (int c = c0; c < c1; ++c, ++it) {
                 const int st = it % C::STAGES, n = it / C::STAGES;
                 ok = warp_all(mb_wait(&full[st], (uint32_t)n & 1u, p.status, kWaitStage));
@@ -332,20 +300,18 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
                     if constexpr (C::FP4) {
                         const uint32_t sf = b0 + (C::B_BYTES >> 4), ts = sf_tmem + (it & 1) * C::SF_COLS;
                         const int left = p.K - c * C::BK, kbs = left > 128 ? 2 : 1, steps = left >= C::BK ? 4 : (left + 63) >> 6;
-                        // TMEM: A's scales 4 columns per (A, 128 of K), B's 4 per (128 of K, 128 rows)
+                        // TMEM: A's scales 4 columns per (A, 128 of K), B's 4 per 128 of K
                         for (int kb = 0; kb < kbs; ++kb) {
 #pragma unroll
                             for (int a = 0; a < C::NA; ++a) scales_to_tmem(ts + a * 8 + kb * 4, (sf + a * 64 + kb * 32) << 4);
-#pragma unroll
-                            for (int i = 0; i < C::SFB_TILES; ++i)
-                                scales_to_tmem(ts + C::NA * 8 + (kb * C::SFB_TILES + i) * 4, (sf + (C::NA + i) * 64 + kb * 32) << 4);
+                            scales_to_tmem(ts + C::NA * 8 + kb * 4, (sf + C::NA * 64 + kb * 32) << 4);
                         }
                         for (int ks = 0; ks < steps; ++ks) {
                             const uint32_t id = idesc | ((uint32_t)(ks & 1) << 30) | ((uint32_t)(ks & 1) << 5);  // scales 0, 1 or 2, 3 of a word
-                            const uint32_t tb = ts + C::NA * 8 + (ks >> 1) * C::SFB_TILES * 4 + n_sf;
+                            const uint32_t tb = ts + C::NA * 8 + (ks >> 1) * 4;
 #pragma unroll
                             for (int a = 0; a < C::NA; ++a)
-                                mma_mxf4(d + a * C::BN, desc_of((a0 + a * (C::A_BYTES >> 4) + ks * KA) & 0x3FFFu | LA), desc_of((b0 + ks * KB) & 0x3FFFu | LB), id,
+                                mma_mxf4(d + a * C::BN, desc_of(a0 + a * (C::A_BYTES >> 4) + ks * KA | LA), desc_of(b0 + ks * KB | LB), id,
                                          ts + a * 8 + (ks >> 1) * 4, tb, c > c0 || ks > 0);
                         }
                     } else {
@@ -353,7 +319,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
                         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
                             for (int a = 0; a < C::NA; ++a)
-                                mma_bf16(d + a * C::BN, desc_of((a0 + a * (C::A_BYTES >> 4) + ks * KA) & 0x3FFFu | LA), desc_of((b0 + ks * KB) & 0x3FFFu | LB), idesc,
+                                mma_bf16(d + a * C::BN, desc_of(a0 + a * (C::A_BYTES >> 4) + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc,
                                          c > c0 || ks > 0);
                     }
                     mma_commit(&empty[st]);
@@ -371,14 +337,13 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
             ok = warp_all(mb_wait(&tfull[buf], (uint32_t)use & 1u, p.status, kWaitAcc));
             if (!ok) break;
             tc_fence_after();
-            const Tile tl = tile_of<C>(p, t);
             const uint32_t tacc = tmem + buf * C::ACC;
             if (p.splits == 1) {
                 switch (p.out_type) {
-                    case T_F32: tile_out<C, T_F32>(p, tl, tacc, quad, half, lane); break;
-                    case T_F16: tile_out<C, T_F16>(p, tl, tacc, quad, half, lane); break;
-                    case T_BF16: tile_out<C, T_BF16>(p, tl, tacc, quad, half, lane); break;
-                    default: if constexpr (C::FP4 && C::NA == 2) tile_out<C, T_MXFP4>(p, tl, tacc, quad, half, lane);
+                    case T_F32: tile_out<C, T_F32>(p, t, tacc, quad, half, lane); break;
+                    case T_F16: tile_out<C, T_F16>(p, t, tacc, quad, half, lane); break;
+                    case T_BF16: tile_out<C, T_BF16>(p, t, tacc, quad, half, lane); break;
+                    default: if constexpr (C::FP4 && C::NA == 2) tile_out<C, T_MXFP4>(p, t, tacc, quad, half, lane);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -402,13 +367,12 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
         cluster_sync();
         if (warp >= 2) {
             const int quad = warp & 3, half = (warp - 2) >> 2;
-            const Tile tl = tile_of<C>(p, first);
             const uint32_t red = s32(smem);
             switch (p.out_type) {
-                case T_F32: split_out<C, T_F32>(p, tl, red, rank, quad, half, lane); break;
-                case T_F16: split_out<C, T_F16>(p, tl, red, rank, quad, half, lane); break;
-                case T_BF16: split_out<C, T_BF16>(p, tl, red, rank, quad, half, lane); break;
-                default: if constexpr (C::FP4 && C::NA == 2) split_out<C, T_MXFP4>(p, tl, red, rank, quad, half, lane);
+                case T_F32: split_out<C, T_F32>(p, first, red, rank, quad, half, lane); break;
+                case T_F16: split_out<C, T_F16>(p, first, red, rank, quad, half, lane); break;
+                case T_BF16: split_out<C, T_BF16>(p, first, red, rank, quad, half, lane); break;
+                default: if constexpr (C::FP4 && C::NA == 2) split_out<C, T_MXFP4>(p, first, red, rank, quad, half, lane);
             }
         }
         __syncwarp();
@@ -427,29 +391,23 @@ struct Operand {  // a matrix in memory
     const void* data;
     uint64_t rows, cols, pitch;  // pitch: bytes between rows
 };
-template <class C>
+template <bool FP4>
 int operand_map(CUtensorMap* m, const Operand& o, int box_rows, int type) {
-    if constexpr (C::FP4) return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.data, o.rows, o.cols / 2, o.pitch, box_rows);
+    if constexpr (FP4) return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.data, o.rows, o.cols / 2, o.pitch, box_rows);
     return tiled_map(m, type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.data, o.rows, o.cols, o.pitch, box_rows);
 }
 
-// p: everything but the maps and the tiles.  a, b: C::NA or p.passes operands of A, p.passes or p.both of B.
+// p: everything but the maps, the operands' type and the splits.  a, b: C::NA or p.passes operands of A, p.passes of B.
 template <class C>
 int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* b, int nb, int type, const char* name) {
     int rc;
     for (int i = 0; i < na; ++i)
-        if ((rc = operand_map<C>(&p.a[i], a[i], C::AMN ? 64 : TM, type))) return rc;
+        if ((rc = operand_map<C::FP4>(&p.a[i], a[i], C::AMN ? 64 : TM, type))) return rc;
     for (int i = 0; i < nb; ++i)
-        if ((rc = operand_map<C>(&p.b[i], b[i], C::BMN ? 64 : C::BN, type))) return rc;
+        if ((rc = operand_map<C::FP4>(&p.b[i], b[i], C::BN, type))) return rc;
     p.idesc_type = type == T_BF16;
     p.status = c->status;
-    p.tiles_m = (p.M + TM - 1) / TM;
-    p.tiles_n = (p.N + C::BN - 1) / C::BN;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.both, chunks = (int64_t)((p.K + C::BK - 1) / C::BK) * p.passes;
-    if (tiles > 0x3fffffff) {
-        set_error("%s: %d x %d results are more than one launch takes", name, p.N, p.M);
-        return DNB_DECLINED;
-    }
+    const int tiles = (p.M + TM - 1) / TM, chunks = (p.K + C::BK - 1) / C::BK * p.passes;
     static_assert(C::ACC * TM * 4 <= C::STAGES * C::STAGE, "the partial sums of a split lie in the ring");
     const int slots = c->sm_count * C::PER_SM;
     p.splits = 1;

@@ -8,11 +8,13 @@
 // No operand is transposed in memory: the tensor core takes G, U, x, dg and du from shared memory with either index innermost.
 // Kept from the forward pass are g and u, in 32 bits: rounded to 16, dg and du would be off by twice their own rounding.
 // dg and du are rounded to the operands' type, as the tensor cores take them; all sums are 32 bits.
-#include "dense_tc.cuh"
+#include "dense_pair.cuh"
 
 namespace dnb {
 namespace gt {
 using namespace dt;
+using dt::Cfg;
+using dt::Params;
 
 __device__ __forceinline__ void act_and_slope(int act, float g, float& a, float& slope) {
     if (act == ACT_SILU) {
@@ -110,20 +112,33 @@ int dnb_gated_dev(dnb_ctx* c, int act, int type, const void* x_dev, size_t ldx, 
         return DNB_DECLINED;
     }
     DNB_CUDA(cudaSetDevice(c->device));
+    const uint64_t N = n, K = k, T = nt;
+    const Operand w[2] = {{gate_dev, N, K, K * 2}, {up_dev, N, K, K * 2}}, x = {x_dev, T, K, (uint64_t)ldx * 2};
+    if (nt > 128) {
+        dp::Params p = {};
+        p.M = nt; p.N = n; p.K = k;
+        p.passes = p.both = 1;
+        p.outp[0] = out_dev;
+        p.out_type = type;
+        p.ldo = ldo;
+        p.act = act;
+        p.keep = pre_dev != nullptr;
+        for (int i = 0; i < 2 && p.keep; ++i)
+            if ((rc = dp::result_map(&p.pre[i], T_F32, pre_dev + i * T * N, T, N, N))) return rc;
+        return dp::launch_pair<dp::Cfg<false, true>>(c, p, &x, 1, w, 2, type, "gated");
+    }
     Params p = {};
     p.M = n; p.N = nt; p.K = k;
-    p.passes = p.both = 1;
-    p.out[0] = out_dev;
+    p.passes = 1;
+    p.out = out_dev;
     p.out_type = type;
     p.ldo = ldo;
     p.act = act;
     p.pre = pre_dev;
-    const Operand a[2] = {{gate_dev, (uint64_t)n, (uint64_t)k, (uint64_t)k * 2}, {up_dev, (uint64_t)n, (uint64_t)k, (uint64_t)k * 2}};
-    const Operand b = {x_dev, (uint64_t)nt, (uint64_t)k, (uint64_t)ldx * 2};
-    if (nt <= 16) return launch_dense<Cfg<false, 2, 16>>(c, p, a, 2, &b, 1, type, "gated");
-    if (nt <= 32) return launch_dense<Cfg<false, 2, 32>>(c, p, a, 2, &b, 1, type, "gated");
-    if (nt <= 64) return launch_dense<Cfg<false, 2, 64>>(c, p, a, 2, &b, 1, type, "gated");
-    return launch_dense<Cfg<false, 2, 128>>(c, p, a, 2, &b, 1, type, "gated");
+    if (nt <= 16) return launch_dense<Cfg<false, 2, 16>>(c, p, w, 2, &x, 1, type, "gated");
+    if (nt <= 32) return launch_dense<Cfg<false, 2, 32>>(c, p, w, 2, &x, 1, type, "gated");
+    if (nt <= 64) return launch_dense<Cfg<false, 2, 64>>(c, p, w, 2, &x, 1, type, "gated");
+    return launch_dense<Cfg<false, 2, 128>>(c, p, w, 2, &x, 1, type, "gated");
 }
 
 int dnb_gated_backward_dev(dnb_ctx* c, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev, const float* pre_dev,
@@ -171,32 +186,41 @@ int dnb_gated_backward_dev(dnb_ctx* c, int act, int type, const void* x_dev, siz
     const uint64_t N = n, K = k, T = nt;
     const Operand d[2] = {{dpre, T, N, N * 2}, {dpre + T * N * 2, T, N, N * 2}};
     if (dx_dev) {
-        Params p = {};
-        p.M = k; p.N = nt; p.K = n;
-        p.passes = 2;
-        p.both = 1;
-        p.out[0] = dx_dev;
-        p.out_type = type;
-        p.ldo = lddx;
         const Operand w[2] = {{gate_dev, N, K, K * 2}, {up_dev, N, K, K * 2}};
-        if (nt <= 16) rc = launch_dense<Cfg<false, 1, 16, true>>(c, p, w, 2, d, 2, type, "gated_dx");
-        else if (nt <= 32) rc = launch_dense<Cfg<false, 1, 32, true>>(c, p, w, 2, d, 2, type, "gated_dx");
-        else if (nt <= 64) rc = launch_dense<Cfg<false, 1, 64, true>>(c, p, w, 2, d, 2, type, "gated_dx");
-        else if (nt <= 128) rc = launch_dense<Cfg<false, 1, 128, true>>(c, p, w, 2, d, 2, type, "gated_dx");
-        else rc = launch_dense<Cfg<false, 1, 256, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        if (nt <= 128) {
+            Params p = {};
+            p.M = k; p.N = nt; p.K = n;
+            p.passes = 2;
+            p.out = dx_dev;
+            p.out_type = type;
+            p.ldo = lddx;
+            if (nt <= 16) rc = launch_dense<Cfg<false, 1, 16, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+            else if (nt <= 32) rc = launch_dense<Cfg<false, 1, 32, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+            else if (nt <= 64) rc = launch_dense<Cfg<false, 1, 64, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+            else rc = launch_dense<Cfg<false, 1, 128, true>>(c, p, w, 2, d, 2, type, "gated_dx");
+        } else {
+            dp::Params p = {};
+            p.M = nt; p.N = k; p.K = n;
+            p.passes = 2;
+            p.both = 1;
+            p.outp[0] = dx_dev;
+            p.out_type = type;
+            p.ldo = lddx;
+            rc = dp::launch_pair<dp::Cfg<false, false, false, true>>(c, p, d, 2, w, 2, type, "gated_dx");
+        }
         if (rc) return rc;
     }
     if (weights) {
-        Params p = {};
-        p.M = k; p.N = n; p.K = nt;
+        dp::Params p = {};
+        p.M = n; p.N = k; p.K = nt;
         p.passes = 1;
         p.both = 2;
-        p.out[0] = dgate_dev;
-        p.out[1] = dup_dev;
+        p.outp[0] = dgate_dev;
+        p.outp[1] = dup_dev;
         p.out_type = type;
         p.ldo = k;
         const Operand x = {x_dev, T, K, (uint64_t)ldx * 2};
-        if ((rc = launch_dense<Cfg<false, 1, 256, true, true>>(c, p, &x, 1, d, 2, type, "gated_dw"))) return rc;
+        if ((rc = dp::launch_pair<dp::Cfg<false, false, true, true>>(c, p, d, 2, &x, 1, type, "gated_dw"))) return rc;
     }
     return DNB_OK;
 }

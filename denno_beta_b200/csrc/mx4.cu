@@ -4,11 +4,13 @@
 // from swizzled shared memory, so that TMA moves them as they are.  scales: a byte for each 32 elements of a row, 2^(byte - 127), in tiles of
 // 128 rows x 4 scales of 512 bytes: the order in which tcgen05.cp puts them into tensor memory.  (A GGUF file has both in one block of 17
 // bytes, which neither could take.)
-#include "dense_tc.cuh"
+#include "dense_pair.cuh"
 
 namespace dnb {
 namespace mx {
 using namespace dt;
+using dt::Cfg;
+using dt::Params;
 
 // 16 threads a unit of 128 elements of a row (a scale tile's width), 8 elements a thread; a block of 32 is four neighbouring lanes.
 constexpr int UNIT_THREADS = 16, THREADS = 256, UNITS = THREADS / UNIT_THREADS;
@@ -177,14 +179,41 @@ static int check_matrix(const char* what, const void* codes, const void* scales,
     return DNB_OK;
 }
 
+// One product (NA 1) or the gated one (2).  Up to 128 tokens: narrow tiles of tokens under the weights' rows (dense_tc.cuh); beyond, tiles of
+// 256 tokens (dense_pair.cuh).
 template <int NA>
-static int product(dnb_ctx* c, Params& p, const Operand* a, const Operand* b, const char* name) {
-    if (p.N <= 16) return launch_dense<Cfg<true, NA, 16>>(c, p, a, NA, b, 1, 0, name);
-    if (p.N <= 32) return launch_dense<Cfg<true, NA, 32>>(c, p, a, NA, b, 1, 0, name);
-    if (p.N <= 64) return launch_dense<Cfg<true, NA, 64>>(c, p, a, NA, b, 1, 0, name);
-    if (p.N <= 128 || NA == 2) return launch_dense<Cfg<true, NA, 128>>(c, p, a, NA, b, 1, 0, name);
-    if constexpr (NA == 1) return launch_dense<Cfg<true, 1, 256>>(c, p, a, NA, b, 1, 0, name);
-    return DNB_DECLINED;
+static int product(dnb_ctx* c, const void* xc, const void* xs, const void* const* wc, const void* const* ws, int nt, int k, int n, int act, int type, void* out,
+                   uint8_t* out_scales, size_t ldo, const char* name) {
+    const uint64_t K = k, N = n;
+    const Operand w[2] = {{wc[0], N, K, K / 2}, {wc[NA - 1], N, K, K / 2}}, x = {xc, (uint64_t)nt, K, K / 2};
+    if (nt <= 128) {
+        Params p = {};
+        p.M = n; p.N = nt; p.K = k;
+        p.passes = 1;
+        p.sa[0] = (const uint8_t*)ws[0];
+        p.sa[1] = (const uint8_t*)ws[NA - 1];
+        p.sb = (const uint8_t*)xs;
+        p.out = out;
+        p.out_scales = out_scales;
+        p.out_type = type;
+        p.ldo = ldo;
+        p.act = act;
+        if (nt <= 16) return launch_dense<Cfg<true, NA, 16>>(c, p, w, NA, &x, 1, 0, name);
+        if (nt <= 32) return launch_dense<Cfg<true, NA, 32>>(c, p, w, NA, &x, 1, 0, name);
+        if (nt <= 64) return launch_dense<Cfg<true, NA, 64>>(c, p, w, NA, &x, 1, 0, name);
+        return launch_dense<Cfg<true, NA, 128>>(c, p, w, NA, &x, 1, 0, name);
+    }
+    dp::Params p = {};
+    p.M = nt; p.N = n; p.K = k;
+    p.passes = p.both = 1;
+    p.outp[0] = out;
+    p.out_scales = out_scales;
+    p.out_type = type;
+    p.ldo = ldo;
+    p.act = act;
+    int rc = dp::scale_map(&p.sa, xs, nt, k);
+    for (int i = 0; i < 2 && !rc; ++i) rc = dp::scale_map(&p.sb[i], ws[i < NA ? i : 0], n, k);
+    return rc ? rc : dp::launch_pair<dp::Cfg<true, NA == 2>>(c, p, &x, 1, w, NA, 0, name);
 }
 
 }  // namespace mx
@@ -282,17 +311,7 @@ int dnb_mx4_gemm_dev(dnb_ctx* c, const void* xc, const void* xs, const void* wc,
     }
     if (nt == 0) return DNB_OK;
     DNB_CUDA(cudaSetDevice(c->device));
-    Params p = {};
-    p.M = n; p.N = nt; p.K = k;
-    p.passes = p.both = 1;
-    p.sa[0] = (const uint8_t*)ws;
-    p.sb = (const uint8_t*)xs;
-    p.out[0] = out_dev;
-    p.out_type = type;
-    p.ldo = ldo;
-    p.act = ACT_NONE;
-    const Operand a = {wc, (uint64_t)n, (uint64_t)k, (uint64_t)k / 2}, b = {xc, (uint64_t)nt, (uint64_t)k, (uint64_t)k / 2};
-    return product<1>(c, p, &a, &b, "mx4_gemm");
+    return product<1>(c, xc, xs, &wc, &ws, nt, k, n, ACT_NONE, type, out_dev, nullptr, ldo, "mx4_gemm");
 }
 
 int dnb_mx4_gated_dev(dnb_ctx* c, int act, const void* xc, const void* xs, const void* gc, const void* gs, const void* uc, const void* us, int nt, int k,
@@ -313,20 +332,8 @@ int dnb_mx4_gated_dev(dnb_ctx* c, int act, const void* xc, const void* xs, const
     }
     if (nt == 0) return DNB_OK;
     DNB_CUDA(cudaSetDevice(c->device));
-    Params p = {};
-    p.M = n; p.N = nt; p.K = k;
-    p.passes = p.both = 1;
-    p.sa[0] = (const uint8_t*)gs;
-    p.sa[1] = (const uint8_t*)us;
-    p.sb = (const uint8_t*)xs;
-    p.out[0] = out_dev;
-    p.out_scales = (uint8_t*)out_scales_dev;
-    p.out_type = type;
-    p.ldo = ldo;
-    p.act = act;
-    const Operand a[2] = {{gc, (uint64_t)n, (uint64_t)k, (uint64_t)k / 2}, {uc, (uint64_t)n, (uint64_t)k, (uint64_t)k / 2}};
-    const Operand b = {xc, (uint64_t)nt, (uint64_t)k, (uint64_t)k / 2};
-    return product<2>(c, p, a, &b, "mx4_gated");
+    const void *wc[2] = {gc, uc}, *ws[2] = {gs, us};
+    return product<2>(c, xc, xs, wc, ws, nt, k, n, act, type, out_dev, (uint8_t*)out_scales_dev, ldo, "mx4_gated");
 }
 
 }  // extern "C"
