@@ -8,7 +8,7 @@
 //
 // A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight
 // warps read the accumulators: a thread a row, 32 columns at a time, through 4 KB of shared memory a warp and out by TMA stores (or, where
-// rows do not start at multiples of 16 bytes, in whole rows by plain stores).  16 bits: two accumulators; 4 bits, where the scales take the
+// rows do not start or end at multiples of 16 bytes, in whole rows by plain stores).  16 bits: two accumulators; 4 bits, where the scales take the
 // room: one, drained to registers at once so that the next tile's MMAs need not wait for the stores.
 #pragma once
 #include "dense_tc.cuh"
@@ -116,44 +116,53 @@ __device__ __forceinline__ uint32_t two(float a, float b) {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
-// 32 rows x 32 columns of a warp, a row a lane, from (row0, col0) of a [M][N] matrix.  buf: the warp's 4 KB; rows of 64 or 128 bytes in the
-// swizzle of the tensor map, which keeps the 16-byte stores of eight lanes apart.
+// A warp's 32 rows x 128 bytes of results, a row a lane, in its 4 KB of shared memory, 16 bytes swizzled as in the tensor map (which keeps the
+// stores of eight lanes apart), and out as one box: rows of 128 bytes, as TMA's stores go by the row.
+__device__ __forceinline__ void chunk_put(uint8_t* buf, int lane, const float (&v)[32]) {
+    uint8_t* row = buf + lane * 128;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<float4*>(row + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+__device__ __forceinline__ void chunk_put(uint8_t* buf, int lane, int part, const uint32_t (&h)[16]) {  // 16 bits: one of two halves of a row
+    uint8_t* row = buf + lane * 128;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(row + (((c + 4 * part) ^ (lane & 7)) << 4)) = make_uint4(h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+}
 template <int OUT>
-__device__ __forceinline__ void chunk_out(const CUtensorMap* map, bool tma, void* out, size_t ldo, int M, int N, int row0, int col0, const float (&v)[32], uint8_t* buf,
-                                          int lane) {
-    if (row0 >= M || col0 >= N) return;  // the whole warp
-    if (tma) {
-        if (lane == 0) store_read();
-    }
+__device__ __forceinline__ void halves(const float (&v)[32], uint32_t (&h)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) h[i] = two<OUT>(v[2 * i], v[2 * i + 1]);
+}
+// Before chunk_put: the last box has been read.
+__device__ __forceinline__ void chunk_begin(int lane) {
+    if (lane == 0) store_read();
     __syncwarp();
-    if constexpr (OUT == T_F32) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-    } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(two<OUT>(v[8 * c], v[8 * c + 1]), two<OUT>(v[8 * c + 2], v[8 * c + 3]), two<OUT>(v[8 * c + 4], v[8 * c + 5]), two<OUT>(v[8 * c + 6], v[8 * c + 7]));
-    }
+}
+// From (row0, col0) of a [M][N] matrix.
+template <int OUT>
+__device__ __forceinline__ void chunk_end(const CUtensorMap* map, bool tma, void* out, size_t ldo, int M, int N, int row0, int col0, uint8_t* buf, int lane) {
     if (tma) {
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) store_2d(map, col0, row0, s32(buf));
-    } else {
-        __syncwarp();
-        if (col0 + lane < N) {
-            const int rows = min(32, M - row0);
-            for (int r = 0; r < rows; ++r) {
-                const size_t at = (size_t)(row0 + r) * ldo + col0 + lane;
-                if constexpr (OUT == T_F32)
-                    reinterpret_cast<float*>(out)[at] = *reinterpret_cast<const float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                else
-                    reinterpret_cast<uint16_t*>(out)[at] = *reinterpret_cast<const uint16_t*>(buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-            }
-        }
-        __syncwarp();
+        if (lane == 0 && row0 < M && col0 < N) store_2d(map, col0, row0, s32(buf));
+        return;
     }
+    __syncwarp();
+    const int rows = min(32, M - row0);
+    constexpr int SIZE = OUT == T_F32 ? 4 : 2;
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+#pragma unroll
+        for (int i = 0; i < 4 / SIZE; ++i) {
+            const int c = 32 * i + lane;
+            if (col0 + c >= N) continue;
+            const uint8_t* src = buf + r * 128 + (((c * SIZE >> 4) ^ (r & 7)) << 4) + (c * SIZE & 15);
+            const size_t at = (size_t)(row0 + r) * ldo + col0 + c;
+            if constexpr (OUT == T_F32) reinterpret_cast<float*>(out)[at] = *reinterpret_cast<const float*>(src);
+            else reinterpret_cast<uint16_t*>(out)[at] = *reinterpret_cast<const uint16_t*>(src);
+        }
+    }
+    __syncwarp();
 }
 // 32 features of a row as one 4-bit block.
 __device__ __forceinline__ void block_out(const Params& p, int row, int col, const float (&v)[32]) {
@@ -173,14 +182,49 @@ __device__ __forceinline__ void block_out(const Params& p, int row, int col, con
     p.out_scales[scale_at(row, col >> 5, (p.N + 127) >> 7)] = (uint8_t)(col < p.N ? e : 0u);
 }
 
+// What a thread does with 32 columns (gated: of g and of u) from `col`: chunk c of its row.
+template <class C, int OUT>
+__device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which, int c, int row0, int col, float (&g)[32], float (&u)[32], uint8_t* buf, int lane,
+                                         uint32_t (&first)[16]) {
+    if constexpr (C::GATED) {
+        if (p.keep) {
+            chunk_begin(lane);
+            chunk_put(buf, lane, g);
+            chunk_end<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
+            chunk_begin(lane);
+            chunk_put(buf, lane, u);
+            chunk_end<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) g[j] = act_of(act, g[j]) * u[j];
+    }
+    if constexpr (OUT == T_MXFP4) {
+        block_out(p, row0 + lane, col, g);
+    } else if constexpr (OUT == T_F32) {
+        chunk_begin(lane);
+        chunk_put(buf, lane, g);
+        chunk_end<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col, buf, lane);
+    } else {
+        // two chunks make a row of 128 bytes; the buffer may be wanted for pre between them
+        if ((c & 1) == 0) return halves<OUT>(g, first);
+        uint32_t h[16];
+        halves<OUT>(g, h);
+        chunk_begin(lane);
+        chunk_put(buf, lane, 0, first);
+        chunk_put(buf, lane, 1, h);
+        chunk_end<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col - 32, buf, lane);
+    }
+}
+
 template <class C, int OUT>
 __device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t* buf, int lane, uint32_t drained) {
-    // This thread's columns: 32 at a time; gated: 32 of gate and of up.
     constexpr int CHUNKS = C::GATED ? 2 : 4;
-    constexpr bool DRAIN = C::BUFS == 1;
-    float v[DRAIN ? 4 : C::GATED ? 2 : 1][32];
-    const int at = half * (C::GATED ? 64 : 128);
-    if constexpr (DRAIN) {
+    const int at = half * 32 * CHUNKS;
+    const ActForm act = act_form(p.act);
+    uint32_t first[16];
+    if constexpr (C::BUFS == 1) {
+        // drained to registers: every element of them by a constant index, so the chunks are unrolled
+        float v[4][32];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             tmem_ld32(ta + at + 32 * c, v[c]);
@@ -190,30 +234,23 @@ __device__ __forceinline__ void results(const Params& p, int which, int row0, in
         tc_fence_before();
         __syncwarp();
         if (lane == 0) remote_arrive(drained);
-    }
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const int g = DRAIN ? c : 0, u = DRAIN ? 2 + c : C::GATED ? 1 : 0, col = n0 + at + 32 * c;
-        if constexpr (!DRAIN) {
-            tmem_ld32(ta + at + 32 * c, v[0]);
-            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, v[1]);
+        for (int c = 0; c < CHUNKS; ++c) chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, v[c], v[C::GATED ? 2 + c : c], buf, lane, first);
+    } else {
+        // one chunk's code: unrolled, it would not fit the instruction cache
+#pragma unroll 1
+        for (int c = 0; c < CHUNKS; ++c) {
+            float g[32], u[32];
+            tmem_ld32(ta + at + 32 * c, g);
+            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, u);
             tmem_ld_wait();
-        }
-        if constexpr (C::GATED) {
-            if (p.keep) {
-                chunk_out<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, v[g], buf, lane);
-                chunk_out<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, v[u], buf, lane);
+            if (c == CHUNKS - 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) remote_arrive(drained);
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[g][j] = act_of(p.act, v[g][j]) * v[u][j];
+            chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, g, u, buf, lane, first);
         }
-        if constexpr (OUT == T_MXFP4) block_out(p, row0 + lane, col, v[g]);
-        else chunk_out<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col, v[g], buf, lane);
-    }
-    if constexpr (!DRAIN) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) remote_arrive(drained);
     }
 }
 
@@ -389,11 +426,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
 inline int scale_map(CUtensorMap* m, const void* scales, uint64_t rows, uint64_t k) {
     return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, scales, (rows + 127) / 128 * ((k + 127) / 128), 128, 512, 2, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-// Results [rows][cols] of `type`, in the epilogue's chunks.
+// Results [rows][cols] of `type`, in the epilogue's boxes.
 inline int result_map(CUtensorMap* m, int type, const void* out, uint64_t rows, uint64_t cols, uint64_t ld) {
     const bool f32 = type == T_F32;
     return tiled_map(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, f32 ? 4 : 2, out, rows,
-                     cols, ld * (f32 ? 4 : 2), 32, 32, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                     cols, ld * (f32 ? 4 : 2), 32);
 }
 
 // p: M, N, K, passes, both, type, act, outp, out_scales, ldo; maps of scales and pre where there are any.

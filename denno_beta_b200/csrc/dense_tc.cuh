@@ -67,11 +67,14 @@ struct Cfg {
     static_assert(!FP4 || !AMN, "4-bit operands lie along K");
 };
 
-__device__ __forceinline__ float act_of(int act, float g) {
-    if (act == ACT_SILU) return g / (1.f + __expf(-g));
-    const float t = tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g));
-    return 0.5f * g * (1.f + t);
+// Both activations are g / (1 + exp(-z)) with z = g (c0 + c1 g^2): silu has z = g, and v / 2 (1 + tanh(y)) = v / (1 + exp(-2 y)).  No branch,
+// two special functions; the approximate exponential and quotient are off by a few steps of 32 bits.
+struct ActForm { float c0, c1; };
+__device__ __forceinline__ ActForm act_form(int act) {
+    return act == ACT_SILU ? ActForm{1.f, 0.f} : ActForm{1.5957691216057308f, 1.5957691216057308f * 0.044715f};
 }
+__device__ __forceinline__ float act_square(float g) { return fminf(g * g, 1e30f); }  // finite, so that 0 times it is 0
+__device__ __forceinline__ float act_of(ActForm f, float g) { return __fdividef(g, 1.f + __expf(-g * fmaf(f.c1, act_square(g), f.c0))); }
 
 template <int OUT>
 __device__ __forceinline__ void put(void* out, size_t at, float v) {
@@ -141,7 +144,7 @@ template <class C, int OUT>
 __device__ __forceinline__ void emit(const Params& p, int m, int n, float v0, float v1) {
     float v = v0;
     if constexpr (C::NA == 2) {
-        v = act_of(p.act, v0) * v1;
+        v = act_of(act_form(p.act), v0) * v1;
         if (p.pre && m < p.M) {
             p.pre[(size_t)n * p.M + m] = v0;
             p.pre[((size_t)p.N + n) * p.M + m] = v1;

@@ -16,24 +16,20 @@ using namespace dt;
 using dt::Cfg;
 using dt::Params;
 
-__device__ __forceinline__ void act_and_slope(int act, float g, float& a, float& slope) {
-    if (act == ACT_SILU) {
-        const float p = 1.f / (1.f + __expf(-g));
-        a = g * p;
-        slope = p * (1.f + g * (1.f - p));
-    } else {
-        const float t = tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g));
-        a = 0.5f * g * (1.f + t);
-        slope = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * 0.7978845608028654f * (1.f + 0.134145f * g * g);
-    }
+// With p = 1 / (1 + exp(-z)): act = g p, act' = p + g p (1 - p) z'.
+__device__ __forceinline__ void act_and_slope(ActForm f, float g, float& a, float& slope) {
+    const float s = act_square(g), p = __fdividef(1.f, 1.f + __expf(-g * fmaf(f.c1, s, f.c0)));
+    a = g * p;
+    slope = p + a * (1.f - p) * fmaf(3.f * f.c1, s, f.c0);
 }
 
 // Eight features a thread: pre [2][nt][n] fp32, dout rows ldd apart, dpre [2][nt][n].
 template <int T>
 __global__ void __launch_bounds__(256)
-gradients_kernel(int act, const float* __restrict__ pre, const void* __restrict__ dout, size_t ldd, int nt, int n, void* __restrict__ dpre) {
+gradients_kernel(int act_id, const float* __restrict__ pre, const void* __restrict__ dout, size_t ldd, int nt, int n, void* __restrict__ dpre) {
     pdl_wait();
     pdl_launch_dependents();
+    const ActForm act = act_form(act_id);
     const size_t per = n / 8, all = per * nt, plane = (size_t)nt * n;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
         const size_t t = i / per, at = (i - t * per) * 8;
