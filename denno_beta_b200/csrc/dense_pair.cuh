@@ -40,8 +40,9 @@ struct Cfg {
     static constexpr int HALF = 128 * 128;                     // a CTA's half of an operand's tile
     static constexpr int SF = FP4 ? 3 * 1024 : 0;              // scales: 128 rows of A, 256 of B, 256 of K
     static constexpr int STAGE = 2 * HALF + SF;
-    static constexpr int STAGES = FP4 ? 5 : 6;
-    static constexpr int STAGING = EPI_WARPS * 4096;
+    static constexpr int STAGES = 5;
+    static constexpr int BOXES = FP4 ? 1 : 2;                  // 4 KB of results a warp may have on their way
+    static constexpr int STAGING = EPI_WARPS * BOXES * 4096;
     static constexpr int ACC = 256, BUFS = FP4 ? 1 : 2;
     static constexpr int SF_COLS = 24;                         // 8 of A, 16 of B
     static constexpr int COLS = 512;
@@ -64,7 +65,8 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, u
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+template <int MORE>
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(MORE) : "memory"); }
 __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -133,9 +135,11 @@ __device__ __forceinline__ void halves(const float (&v)[32], uint32_t (&h)[16]) 
 #pragma unroll
     for (int i = 0; i < 16; ++i) h[i] = two<OUT>(v[2 * i], v[2 * i + 1]);
 }
-// Before chunk_put: the last box has been read.
-__device__ __forceinline__ void chunk_begin(int lane) {
-    if (lane == 0) store_read();
+// Before chunk_put: another of the warp's boxes, which has been read by now.
+template <class C>
+__device__ __forceinline__ void chunk_begin(int lane, uint8_t*& buf) {
+    if constexpr (C::BOXES == 2) buf = reinterpret_cast<uint8_t*>(reinterpret_cast<uintptr_t>(buf) ^ 4096);
+    if (lane == 0) store_read<C::BOXES - 1>();
     __syncwarp();
 }
 // From (row0, col0) of a [M][N] matrix.
@@ -184,14 +188,14 @@ __device__ __forceinline__ void block_out(const Params& p, int row, int col, con
 
 // What a thread does with 32 columns (gated: of g and of u) from `col`: chunk c of its row.
 template <class C, int OUT>
-__device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which, int c, int row0, int col, float (&g)[32], float (&u)[32], uint8_t* buf, int lane,
+__device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which, int c, int row0, int col, float (&g)[32], float (&u)[32], uint8_t*& buf, int lane,
                                          uint32_t (&first)[16]) {
     if constexpr (C::GATED) {
         if (p.keep) {
-            chunk_begin(lane);
+            chunk_begin<C>(lane, buf);
             chunk_put(buf, lane, g);
             chunk_end<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
-            chunk_begin(lane);
+            chunk_begin<C>(lane, buf);
             chunk_put(buf, lane, u);
             chunk_end<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
         }
@@ -201,7 +205,7 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
     if constexpr (OUT == T_MXFP4) {
         block_out(p, row0 + lane, col, g);
     } else if constexpr (OUT == T_F32) {
-        chunk_begin(lane);
+        chunk_begin<C>(lane, buf);
         chunk_put(buf, lane, g);
         chunk_end<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col, buf, lane);
     } else {
@@ -209,7 +213,7 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
         if ((c & 1) == 0) return halves<OUT>(g, first);
         uint32_t h[16];
         halves<OUT>(g, h);
-        chunk_begin(lane);
+        chunk_begin<C>(lane, buf);
         chunk_put(buf, lane, 0, first);
         chunk_put(buf, lane, 1, h);
         chunk_end<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col - 32, buf, lane);
@@ -217,7 +221,7 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
 }
 
 template <class C, int OUT>
-__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t* buf, int lane, uint32_t drained) {
+__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t*& buf, int lane, uint32_t drained) {
     constexpr int CHUNKS = C::GATED ? 2 : 4;
     const int at = half * 32 * CHUNKS;
     const ActForm act = act_form(p.act);
@@ -393,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
     } else {
         // ---------------- results ----------------
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        uint8_t* buf_s = staging + (warp - 2) * 4096;
+        uint8_t* buf_s = staging + (warp - 2) * C::BOXES * 4096;
         int nt = 0;
         for (int t = first; t < tiles && ok; t += step, ++nt) {
             const int buf = nt % C::BUFS, use = nt / C::BUFS;

@@ -133,9 +133,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_float(uint32_t smem, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(smem), "r"(rank) : "memory");
+__device__ __forceinline__ float4 peer_floats(uint32_t smem, uint32_t rank) {
+    float4 v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem), "r"(rank) : "memory");
     return v;
 }
 
@@ -185,16 +186,57 @@ __device__ __forceinline__ void tile_out(const Params& p, int tile, uint32_t tac
     }
 }
 
+// The sum of a column's shares, in rank order: a warp a column, four neighbouring features a lane, all shares asked for at once.
 template <class C, int OUT>
-__device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t red, uint32_t rank, int quad, int half, int lane) {
-    const int m = tile * TM + quad * 32 + lane;
-    for (int c = (int)rank + p.splits * half; c < p.N; c += 2 * p.splits) {
-        float s0 = 0.f, s1 = 0.f;
-        for (int r = 0; r < p.splits; ++r) {
-            s0 += peer_float(red + 4u * (uint32_t)(c * TM + quad * 32 + lane), r);
-            if constexpr (C::NA == 2) s1 += peer_float(red + 4u * (uint32_t)((C::BN + c) * TM + quad * 32 + lane), r);
+__device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t red, uint32_t rank, int warp, int lane) {
+    const int m = tile * TM + 4 * lane;
+    const ActForm act = act_form(p.act);
+#pragma unroll 1
+    for (int c = (int)rank + p.splits * warp; c < p.N; c += EPI_WARPS * p.splits) {
+        float4 v[C::NA][8];
+#pragma unroll
+        for (int a = 0; a < C::NA; ++a)
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < p.splits) v[a][r] = peer_floats(red + 4u * (uint32_t)((a * C::BN + c) * TM + 4 * lane), r);
+        float4 s[C::NA];
+#pragma unroll
+        for (int a = 0; a < C::NA; ++a) {
+            s[a] = v[a][0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r)
+                if (r < p.splits) {
+                    s[a].x += v[a][r].x; s[a].y += v[a][r].y; s[a].z += v[a][r].z; s[a].w += v[a][r].w;
+                }
         }
-        emit<C, OUT>(p, m, c, s0, s1);
+        float o[4] = {s[0].x, s[0].y, s[0].z, s[0].w};
+        if constexpr (C::NA == 2) {
+            const float u[4] = {s[1].x, s[1].y, s[1].z, s[1].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (p.pre && m + i < p.M) {
+                    p.pre[(size_t)c * p.M + m + i] = o[i];
+                    p.pre[((size_t)p.N + c) * p.M + m + i] = u[i];
+                }
+                o[i] = act_of(act, o[i]) * u[i];
+            }
+        }
+        if constexpr (OUT == T_MXFP4) {  // a block is eight lanes
+            uint32_t mx = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(o[i]) & 0x7fffffffu);
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const uint32_t e = scale_byte(mx);
+            const float by = scale_inverse(e);
+            const uint32_t code = e2m1_pair(o[0] * by, o[1] * by) | e2m1_pair(o[2] * by, o[3] * by) << 8;
+            if (m < p.M) *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.out) + ((size_t)c * p.M + m) / 2) = (uint16_t)(e == 255 ? 0u : code);
+            if ((lane & 7) == 0) p.out_scales[scale_at(c, m >> 5, (p.M + 127) >> 7)] = (uint8_t)(m < p.M ? e : 0u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (m + i < p.M) put<OUT>(p.out, (size_t)c * p.ldo + m + i, o[i]);
+        }
     }
 }
 
@@ -369,13 +411,12 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
     if (p.splits > 1) {
         cluster_sync();
         if (warp >= 2) {
-            const int quad = warp & 3, half = (warp - 2) >> 2;
             const uint32_t red = s32(smem);
             switch (p.out_type) {
-                case T_F32: split_out<C, T_F32>(p, first, red, rank, quad, half, lane); break;
-                case T_F16: split_out<C, T_F16>(p, first, red, rank, quad, half, lane); break;
-                case T_BF16: split_out<C, T_BF16>(p, first, red, rank, quad, half, lane); break;
-                default: if constexpr (C::FP4 && C::NA == 2) split_out<C, T_MXFP4>(p, first, red, rank, quad, half, lane);
+                case T_F32: split_out<C, T_F32>(p, first, red, rank, warp - 2, lane); break;
+                case T_F16: split_out<C, T_F16>(p, first, red, rank, warp - 2, lane); break;
+                case T_BF16: split_out<C, T_BF16>(p, first, red, rank, warp - 2, lane); break;
+                default: if constexpr (C::FP4 && C::NA == 2) split_out<C, T_MXFP4>(p, first, red, rank, warp - 2, lane);
             }
         }
         __syncwarp();
