@@ -441,6 +441,61 @@ int operand_map(CUtensorMap* m, const Operand& o, int box_rows, int type) {
     return tiled_map(m, type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.data, o.rows, o.cols, o.pitch, box_rows);
 }
 
+template <class C>
+cudaLaunchConfig_t launch_config(dnb_ctx* c, cudaLaunchAttribute (&at)[2], unsigned grid, int splits) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(NTHREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = c->stream;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = c->use_pdl;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = splits;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = splits > 1 ? 2 : 1;
+    return cfg;
+}
+
+// How many clusters of `splits` blocks the device holds at once: blocks of a cluster share a GPC, whose SMs they may not fill (16 clusters of eight
+// where 148 SMs could hold 18).  Asked once a device.
+template <class C>
+int clusters_at_once(dnb_ctx* c, int splits) {
+    static std::atomic<int> known[64][9];
+    std::atomic<int>& k = known[c->device & 63][splits];
+    int n = k.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchAttribute at[2];
+        cudaLaunchConfig_t cfg = launch_config<C>(c, at, splits, splits);
+        if (splits == 1) n = c->sm_count * C::PER_SM;
+        else if (cudaOccupancyMaxActiveClusters(&n, dense_kernel<C>, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 1;
+        }
+        k.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// Into how many parts K is split.  A block costs its chunks of K and, in chunks, what starting and joining it takes (about 100 KB of weights' time);
+// a second block on an SM costs 0.85 of another turn, as an SM's share of the memory's rate is nearly that of one block; another wave costs a whole
+// turn.  us a call for 1 to 8 parts: 4 tokens, 4096 -> 10240 gated in bf16 (80 tiles) 36, 39, 33, 39, 35, 35, 40, 38; dx of 77 tokens (17 tiles, one
+// block an SM) - , -, 32, 28, 25, 24, 36, 34 (beyond 6 parts the clusters take two waves); 4-bit 12288 -> 4096 (32 tiles) -, -, 9.7, 8.5, 8.6, 8.3, 7.8, 7.6.
+template <class C>
+int best_splits(dnb_ctx* c, int tiles, int chunks) {
+    const float start = 100.f * 1024.f / C::STAGE;
+    int best = 1;
+    float least = 0.f;
+    for (int s = 1; s <= 8 && s <= chunks; ++s) {
+        const int at_once = clusters_at_once<C>(c, s), waves = (tiles + at_once - 1) / at_once, blocks = (tiles < at_once ? tiles : at_once) * s;
+        const float turns = 1.f + 0.85f * ((blocks + c->sm_count - 1) / c->sm_count - 1);
+        const float cost = waves * (start + (chunks + s - 1) / s * turns) + 0.15f * s;
+        if (s == 1 || cost < least) best = s, least = cost;
+    }
+    return best;
+}
+
 // p: everything but the maps, the operands' type and the splits.  a, b: C::NA or p.passes operands of A, p.passes of B.
 template <class C>
 int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* b, int nb, int type, const char* name) {
@@ -453,26 +508,14 @@ int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand*
     p.status = c->status;
     const int tiles = (p.M + TM - 1) / TM, chunks = (p.K + C::BK - 1) / C::BK * p.passes;
     static_assert(C::ACC * TM * 4 <= C::STAGES * C::STAGE, "the partial sums of a split lie in the ring");
-    const int slots = c->sm_count * C::PER_SM;
-    p.splits = 1;
-    while (p.splits < 8 && tiles * p.splits * 2 <= slots && chunks >= p.splits * 2) p.splits *= 2;
-    const unsigned grid = p.splits > 1 ? (unsigned)(tiles * p.splits) : (unsigned)(tiles < slots ? tiles : slots);
     static SmemGrant grant;
     DNB_CUDA(grant_smem(grant, c->device, dense_kernel<C>, C::SMEM));
+    p.splits = best_splits<C>(c, tiles, chunks);
+    const int slots = c->sm_count * C::PER_SM;
+    const unsigned grid = p.splits > 1 ? (unsigned)tiles * p.splits : (unsigned)(tiles < slots ? tiles : slots);
     ProfScope prof_(c, c->stream, name);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(NTHREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = c->stream;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = c->use_pdl;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = p.splits;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = p.splits > 1 ? 2 : 1;
+    const cudaLaunchConfig_t cfg = launch_config<C>(c, at, grid, p.splits);
     DNB_CUDA(cudaLaunchKernelEx(&cfg, dense_kernel<C>, p));
     c->launches++;
     return DNB_OK;
