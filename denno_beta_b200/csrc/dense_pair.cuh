@@ -5,6 +5,8 @@
 // Gated: the B tile is 128 rows of gate in one CTA and the same 128 of up in the other, so that a thread that reads a row of D has g and u
 // of the same features: 256 x 128 results from one MMA.
 // Operands as in dense_tc.cuh: 4 bits with scales in tensor memory, or 16 bits with rows along K or along m / n.
+// Tiles go to the pairs in turn.  What is left over when every pair has had as many, or all of them where there are few, one tile a cluster of
+// two or four pairs: these divide K, and each CTA adds up some of the columns, the pairs' shares in ascending order, through distributed shared memory.
 //
 // A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight
 // warps read the accumulators: a thread a row, 32 columns at a time, through 4 KB of shared memory a warp and out by TMA stores (or, where
@@ -25,6 +27,7 @@ struct Params {
     int passes;                     // 2: the sum goes on over a[1], b[1]
     int both;                       // 2: twice the tiles, the second half with a[1] to the second output
     int tiles_m, tiles_n;
+    int parts, whole;               // pairs a cluster; tiles that are not split (the rest: one a cluster)
     int idesc_type, out_type, act;
     bool tma_out, keep;             // keep: g and u to pre
     void* outp[2];
@@ -71,8 +74,8 @@ __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {  // the barrier of both CTAs
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(bar)), "h"((uint16_t)3) : "memory");
+__device__ __forceinline__ void pair_commit(uint64_t* bar, uint16_t pair) {  // the barrier of both CTAs
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(bar)), "h"(pair) : "memory");
 }
 __device__ __forceinline__ void pair_mma16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
@@ -258,6 +261,39 @@ __device__ __forceinline__ void results(const Params& p, int which, int row0, in
     }
 }
 
+// A split tile.  This CTA's sums in the ring's memory, four columns of all rows after another: what a warp reads of another CTA's is 512 bytes in a
+// row (16 bytes a row apart took twice as long).
+__device__ __forceinline__ uint32_t share_at(int row, int unit) { return (uint32_t)(unit * 128 + row) * 16; }
+// 64 columns of the output (a warp 32 rows of them), summed over the cluster's pairs.
+template <class C, int OUT>
+__device__ __forceinline__ void joined(const Params& p, int which, int quad, int row0, int n0, int unit, uint32_t share, uint32_t rank, uint8_t*& buf, int lane) {
+    const ActForm act = act_form(p.act);
+    uint32_t first[16];
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+        const int col = 64 * unit + 32 * c;
+        float v[C::GATED ? 2 : 1][32];
+#pragma unroll
+        for (int a = 0; a < (C::GATED ? 2 : 1); ++a) {
+#pragma unroll 1
+            for (int r = 0; r < p.parts; ++r) {
+                float4 t[8];  // all asked for before the first is added
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = peer_floats(share + share_at(quad * 32 + lane, (a * 128 + col) / 4 + i), 2 * r + rank);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float* s = &v[a][4 * i];
+                    s[0] = r ? s[0] + t[i].x : t[i].x;
+                    s[1] = r ? s[1] + t[i].y : t[i].y;
+                    s[2] = r ? s[2] + t[i].z : t[i].z;
+                    s[3] = r ? s[3] + t[i].w : t[i].w;
+                }
+            }
+        }
+        chunk_of<C, OUT>(p, act, which, c, row0, n0 + col, v[0], v[C::GATED ? 1 : 0], buf, lane, first);
+    }
+}
+
 __device__ __forceinline__ void pair_tile(const Params& p, int t, int& m, int& n, int& which) {
     constexpr int G = 8;  // 8 x 256 rows of A by about as many of B are in flight
     const int per = p.tiles_m * p.tiles_n;
@@ -269,7 +305,7 @@ __device__ __forceinline__ void pair_tile(const Params& p, int t, int& m, int& n
 }
 
 template <class C>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NTHREADS, 1) pair_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* staging = smem + C::STAGES * C::STAGE;
@@ -280,7 +316,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = cluster_rank();
+    const uint32_t in_cluster = cluster_rank(), rank = in_cluster & 1, part = in_cluster >> 1, leader = in_cluster & ~1u;
     if (tid == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
             mb_init(&full[i], 1);   // the leader's: its own expect_tx; bytes of both CTAs
@@ -303,6 +339,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
 
     const int kch = (p.K + C::BK - 1) / C::BK, chunks = kch * p.passes, tiles = p.tiles_m * p.tiles_n * p.both;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    // Turn i of this pair: a tile of its own, or its share of the cluster's tile, which is the last.
+    const int cluster = first / p.parts, own = first < p.whole ? (p.whole - first + step - 1) / step : 0;
+    const bool shares = p.whole + cluster < tiles;
+    const int turns = own + shares, split = p.whole + cluster;
+    const int s0 = (int)((long long)chunks * part / p.parts), s1 = (int)((long long)chunks * (part + 1) / p.parts);
     bool ok = true;
     int m, n, which;
 
@@ -310,17 +351,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
         // ---------------- TMA ----------------
         const int nkb = (p.K + 127) >> 7;
         int it = 0;
-        for (int t = first; t < tiles && ok; t += step) {
-            pair_tile(p, t, m, n, which);
+        for (int i = 0; i < turns && ok; ++i) {
+            pair_tile(p, i < own ? first + i * step : split, m, n, which);
+            const int c0 = i < own ? 0 : s0, c1 = i < own ? chunks : s1;
             const int m0 = m * 256 + (int)rank * 128, n0 = C::GATED ? n * 128 : n * 256 + (int)rank * 128;
-            for (int c = 0; c < chunks; ++c, ++it) {
+            for (int c = c0; c < c1; ++c, ++it) {
                 const int st = it % C::STAGES, use = it / C::STAGES;
                 if (use > 0) ok = warp_all(mb_wait(&empty[st], (uint32_t)(use - 1) & 1u, p.status, kWaitStage));
                 if (!ok) break;
                 if (elect_one()) {
                     uint8_t *sa = smem + st * C::STAGE, *sb = sa + C::HALF;
                     const int pass = c >= kch, kc = pass ? c - kch : c;
-                    const uint32_t bar = in_cta(s32(&full[st]), 0);
+                    const uint32_t bar = in_cta(s32(&full[st]), leader);
                     if (rank == 0) mb_expect_tx(&full[st], 2u * C::STAGE);
                     const CUtensorMap *ma = &p.a[pass | which], *mb = &p.b[C::GATED ? (int)rank : pass];
                     if constexpr (C::AMN) {
@@ -357,14 +399,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
             const uint32_t idesc = C::FP4 ? (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | (1u << 23) | ((256u >> 7) << 27)
                                           : (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) |
                                                 ((uint32_t)C::BMN << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-            int it = 0, nt = 0;
-            for (int t = first; t < tiles && ok; t += step, ++nt) {
+            const uint16_t pair = (uint16_t)(3u << leader);
+            int it = 0;
+            for (int nt = 0; nt < turns && ok; ++nt) {
+                const int c0 = nt < own ? 0 : s0, c1 = nt < own ? chunks : s1;
                 const int buf = nt % C::BUFS, use = nt / C::BUFS;
                 if (use > 0) ok = warp_all(mb_wait(&tempty[buf], (uint32_t)(use - 1) & 1u, p.status, kWaitDrain));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * C::ACC;
-                for (int c = 0; c < chunks; ++c, ++it) {
+                for (int c = c0; c < c1; ++c, ++it) {
                     const int st = it % C::STAGES;
                     ok = warp_all(mb_wait(&full[st], (uint32_t)(it / C::STAGES) & 1u, p.status, kWaitStage));
                     if (!ok) break;
@@ -381,14 +425,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
                             }
                             for (int ks = 0; ks < steps; ++ks)
                                 pair_mma4(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc | ((uint32_t)(ks & 1) << 30) | ((uint32_t)(ks & 1) << 5),
-                                          ts + (ks >> 1) * 4, ts + 8 + (ks >> 1) * 8, c > 0 || ks > 0);
+                                          ts + (ks >> 1) * 4, ts + 8 + (ks >> 1) * 8, c > c0 || ks > 0);
                         } else {
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks)
-                                pair_mma16(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc, c > 0 || ks > 0);
+                                pair_mma16(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc, c > c0 || ks > 0);
                         }
-                        pair_commit(&empty[st]);
-                        if (c == chunks - 1) pair_commit(&tfull[buf]);
+                        pair_commit(&empty[st], pair);
+                        if (c == c1 - 1) pair_commit(&tfull[buf], pair);
                     }
                     __syncwarp();
                 }
@@ -398,15 +442,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
         // ---------------- results ----------------
         const int quad = warp & 3, half = (warp - 2) >> 2;
         uint8_t* buf_s = staging + (warp - 2) * C::BOXES * 4096;
-        int nt = 0;
-        for (int t = first; t < tiles && ok; t += step, ++nt) {
+        for (int nt = 0; nt < turns && ok; ++nt) {
             const int buf = nt % C::BUFS, use = nt / C::BUFS;
             ok = warp_all(mb_wait(&tfull[buf], (uint32_t)use & 1u, p.status, kWaitAcc));
             if (!ok) break;
             tc_fence_after();
-            pair_tile(p, t, m, n, which);
+            const uint32_t ta = tmem + buf * C::ACC + ((uint32_t)(quad * 32) << 16);
+            if (nt == own) {  // the ring is empty: every copy has landed and been read
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float v[32];
+                    tmem_ld32(ta + half * 128 + 32 * c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<float4*>(smem + share_at(quad * 32 + lane, half * 32 + c * 8 + i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+                break;
+            }
+            pair_tile(p, first + nt * step, m, n, which);
             const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
-            const uint32_t ta = tmem + buf * C::ACC + ((uint32_t)(quad * 32) << 16), drained = in_cta(s32(&tempty[buf]), 0);
+            const uint32_t drained = in_cta(s32(&tempty[buf]), leader);
             switch (p.out_type) {
                 case T_F16: results<C, T_F16>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
                 case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
@@ -414,8 +470,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1) pair_ke
                 default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, ta, buf_s, lane, drained);
             }
         }
-        if (lane == 0) store_done();
     }
+    __syncwarp();
+    if (shares) {  // the whole cluster
+        cluster_sync();
+        if (warp >= 2) {
+            const int quad = warp & 3, half = (warp - 2) >> 2, unit = (int)part + half * p.parts;
+            uint8_t* buf_s = staging + (warp - 2) * C::BOXES * 4096;
+            pair_tile(p, split, m, n, which);
+            const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
+            if (unit < C::NOUT / 64) {
+                switch (p.out_type) {
+                    case T_F16: joined<C, T_F16>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane); break;
+                    case T_BF16: joined<C, T_BF16>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane); break;
+                    case T_F32: if constexpr (C::FP4) joined<C, T_F32>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane); break;
+                    default: if constexpr (C::FP4 && C::GATED) joined<C, T_MXFP4>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane);
+                }
+            }
+        }
+    }
+    if (warp >= 2 && lane == 0) store_done();
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // nobody's shared or tensor memory goes while the other may still use it
@@ -435,6 +509,52 @@ inline int result_map(CUtensorMap* m, int type, const void* out, uint64_t rows, 
     const bool f32 = type == T_F32;
     return tiled_map(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, f32 ? 4 : 2, out, rows,
                      cols, ld * (f32 ? 4 : 2), 32);
+}
+
+template <class C>
+cudaLaunchConfig_t pair_config(dnb_ctx* c, cudaLaunchAttribute (&at)[2], unsigned grid, int parts) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(NTHREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = c->stream;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2 * parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = c->use_pdl;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cfg;
+}
+// Clusters of `parts` pairs that the device holds at once (GPCs leave some SMs over).  Asked once a device.
+template <class C>
+int pair_clusters(dnb_ctx* c, int parts) {
+    static std::atomic<int> known[64][5];
+    std::atomic<int>& k = known[c->device & 63][parts];
+    int n = k.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchAttribute at[2];
+        const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2 * parts, parts);
+        if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<C>, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 1;
+        }
+        k.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+// Pairs a cluster and how many tiles are not split.  A tile costs its chunks of K and about four more; a split one a part of the chunks and about
+// ten (shares written, the cluster waited for, sums read).
+template <class C>
+void choose_parts(dnb_ctx* c, int tiles, int chunks, int& parts, int& whole, int& clusters) {
+    float least = 0.f;
+    for (int s = 1; s <= 4; s *= 2) {
+        const int n = pair_clusters<C>(c, s), turns = tiles / (n * s), rest = tiles - turns * n * s;
+        const bool split = s > 1 && rest > 0 && rest <= n && chunks >= s;
+        const float cost = turns * (chunks + 4.f) + (rest == 0 ? 0.f : split ? (float)((chunks + s - 1) / s) + 10.f : chunks + 4.f);
+        if (s == 1 || cost < least) least = cost, parts = s, whole = split ? turns * n * s : tiles, clusters = n;
+    }
 }
 
 // p: M, N, K, passes, both, type, act, outp, out_scales, ldo; maps of scales and pre where there are any.
@@ -461,11 +581,15 @@ int launch_pair(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* 
         set_error("%s: %d x %d results are more than one launch takes", name, p.M, p.N);
         return DNB_DECLINED;
     }
-    const int pairs = c->sm_count / 2;
     static SmemGrant grant;
     DNB_CUDA(grant_smem(grant, c->device, pair_kernel<C>, C::SMEM));
+    int clusters;
+    choose_parts<C>(c, (int)tiles, (p.K + C::BK - 1) / C::BK * p.passes, p.parts, p.whole, clusters);
+    const int used = p.parts == 1 ? (int)tiles : p.whole > 0 ? clusters : (int)tiles;
     ProfScope prof_(c, c->stream, name);
-    DNB_CUDA(launch_k(pair_kernel<C>, dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), dim3(NTHREADS), C::SMEM, c->stream, c->use_pdl, p));
+    cudaLaunchAttribute at[2];
+    const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2u * p.parts * (unsigned)(used < clusters ? used : clusters), p.parts);
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<C>, p));
     c->launches++;
     return DNB_OK;
 }
