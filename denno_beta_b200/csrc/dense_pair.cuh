@@ -6,7 +6,7 @@
 // of the same features: 256 x 128 results from one MMA.
 // Operands as in dense_tc.cuh: 4 bits with scales in tensor memory, or 16 bits with rows along K or along m / n.
 // Tiles go to the pairs in turn.  What is left over when every pair has had as many, or all of them where there are few, one tile a cluster of
-// two or four pairs: these divide K, and each CTA adds up some of the columns, the pairs' shares in ascending order, through distributed shared memory.
+// two to four pairs: these divide K, and each CTA adds up some of the columns, the pairs' shares in ascending order, through distributed shared memory.
 //
 // A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight
 // warps read the accumulators: a thread a row, 32 columns at a time, through 4 KB of shared memory a warp and out by TMA stores (or, where
@@ -549,7 +549,7 @@ int pair_clusters(dnb_ctx* c, int parts) {
 template <class C>
 void choose_parts(dnb_ctx* c, int tiles, int chunks, int& parts, int& whole, int& clusters) {
     float least = 0.f;
-    for (int s = 1; s <= 4; s *= 2) {
+    for (int s = 1; s <= 4; ++s) {
         const int n = pair_clusters<C>(c, s), turns = tiles / (n * s), rest = tiles - turns * n * s;
         const bool split = s > 1 && rest > 0 && rest <= n && chunks >= s;
         const float cost = turns * (chunks + 4.f) + (rest == 0 ? 0.f : split ? (float)((chunks + s - 1) / s) + 10.f : chunks + 4.f);
