@@ -36,6 +36,10 @@ struct Params {
     int* status;
 };
 
+constexpr int PAIR_THREADS = 384;   // a warpgroup for copies and MMAs (two of its warps idle), two for the results
+// Registers after the split, of the 168 a thread that 384 threads start with: 128 x 56 + 256 x 216 = 62,464 of 64,512.
+constexpr int kFewRegs = 56, kManyRegs = 216;
+
 template <bool FP4_, bool GATED_, bool AMN_ = false, bool BMN_ = false>
 struct Cfg {
     static constexpr bool FP4 = FP4_, GATED = GATED_, AMN = AMN_, BMN = BMN_;
@@ -71,8 +75,10 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, u
 template <int MORE>
 __device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(MORE) : "memory"); }
 __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Says that tensor memory has been read (tcgen05.wait::ld and the fence are before it): nothing else has to be visible, and a release at the cluster's
+// scope would wait 1,300 cycles for the stores of the last tile.
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void pair_commit(uint64_t* bar, uint16_t pair) {  // the barrier of both CTAs
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(bar)), "h"(pair) : "memory");
@@ -223,40 +229,30 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
     }
 }
 
+// This thread's part of a tile, 128 columns (gated: 64 of g and of u).  v: drained from tensor memory already, where there is one accumulator.
 template <class C, int OUT>
-__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t*& buf, int lane, uint32_t drained) {
+__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t*& buf, int lane, uint32_t drained, float (&v)[4][32]) {
     constexpr int CHUNKS = C::GATED ? 2 : 4;
     const int at = half * 32 * CHUNKS;
     const ActForm act = act_form(p.act);
     uint32_t first[16];
     if constexpr (C::BUFS == 1) {
-        // drained to registers: every element of them by a constant index, so the chunks are unrolled
-        float v[4][32];
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            tmem_ld32(ta + at + 32 * c, v[c]);
-            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, v[2 + c]);
-        }
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) remote_arrive(drained);
+        // every element by a constant index, so the chunks are unrolled
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, v[c], v[C::GATED ? 2 + c : c], buf, lane, first);
     } else {
         // one chunk's code: unrolled, it would not fit the instruction cache
 #pragma unroll 1
         for (int c = 0; c < CHUNKS; ++c) {
-            float g[32], u[32];
-            tmem_ld32(ta + at + 32 * c, g);
-            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, u);
+            tmem_ld32(ta + at + 32 * c, v[0]);
+            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, v[1]);
             tmem_ld_wait();
             if (c == CHUNKS - 1) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) remote_arrive(drained);
             }
-            chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, g, u, buf, lane, first);
+            chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, v[0], v[1], buf, lane, first);
         }
     }
 }
@@ -305,7 +301,7 @@ __device__ __forceinline__ void pair_tile(const Params& p, int t, int& m, int& n
 }
 
 template <class C>
-__global__ void __launch_bounds__(NTHREADS, 1) pair_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* staging = smem + C::STAGES * C::STAGE;
@@ -347,136 +343,150 @@ __global__ void __launch_bounds__(NTHREADS, 1) pair_kernel(const __grid_constant
     bool ok = true;
     int m, n, which;
 
-    if (warp == 0) {
-        // ---------------- TMA ----------------
-        const int nkb = (p.K + 127) >> 7;
-        int it = 0;
-        for (int i = 0; i < turns && ok; ++i) {
-            pair_tile(p, i < own ? first + i * step : split, m, n, which);
-            const int c0 = i < own ? 0 : s0, c1 = i < own ? chunks : s1;
-            const int m0 = m * 256 + (int)rank * 128, n0 = C::GATED ? n * 128 : n * 256 + (int)rank * 128;
-            for (int c = c0; c < c1; ++c, ++it) {
-                const int st = it % C::STAGES, use = it / C::STAGES;
-                if (use > 0) ok = warp_all(mb_wait(&empty[st], (uint32_t)(use - 1) & 1u, p.status, kWaitStage));
-                if (!ok) break;
-                if (elect_one()) {
-                    uint8_t *sa = smem + st * C::STAGE, *sb = sa + C::HALF;
-                    const int pass = c >= kch, kc = pass ? c - kch : c;
-                    const uint32_t bar = in_cta(s32(&full[st]), leader);
-                    if (rank == 0) mb_expect_tx(&full[st], 2u * C::STAGE);
-                    const CUtensorMap *ma = &p.a[pass | which], *mb = &p.b[C::GATED ? (int)rank : pass];
-                    if constexpr (C::AMN) {
-                        pair_load_2d(sa, ma, m0, kc * 64, bar);
-                        pair_load_2d(sa + 8192, ma, m0 + 64, kc * 64, bar);
-                    } else {
-                        pair_load_2d(sa, ma, kc * (C::FP4 ? 128 : 64), m0, bar);
-                    }
-                    if constexpr (C::BMN) {
-                        pair_load_2d(sb, mb, n0, kc * 64, bar);
-                        pair_load_2d(sb + 8192, mb, n0 + 64, kc * 64, bar);
-                    } else {
-                        pair_load_2d(sb, mb, kc * (C::FP4 ? 128 : 64), n0, bar);
-                    }
-                    if constexpr (C::FP4) {
-                        uint8_t* sf = sb + C::HALF;
-                        pair_load_2d(sf, &p.sa, 0, (m0 >> 7) * nkb + 2 * kc, bar);
-                        pair_load_2d(sf + 1024, &p.sb[0], 0, (C::GATED ? n : 2 * n) * nkb + 2 * kc, bar);
-                        pair_load_2d(sf + 2048, &p.sb[C::GATED], 0, (C::GATED ? n : 2 * n + 1) * nkb + 2 * kc, bar);
-                    }
-                }
-                __syncwarp();
-            }
-        }
-        if (!ok && rank == 0)  // copies in flight, of both CTAs, end before their shared memory is given up
-            for (int i = max(0, it - C::STAGES); i < it; ++i) mb_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
-    } else if (warp == 1) {
-        // ---------------- MMA issue: the leader's thread for both ----------------
-        if (rank == 0) {
-            const uint32_t smem_lo = (s32(smem) & 0x3FFFFu) >> 4;  // in a cluster an address has its CTA's rank above
-            constexpr uint32_t LA = (C::AMN ? (8192u >> 4) : 1u) << 16, LB = (C::BMN ? (8192u >> 4) : 1u) << 16;
-            constexpr uint32_t KA = C::AMN ? 128 : 2, KB = C::BMN ? 128 : 2;
-            const uint32_t sf_tmem = tmem + C::BUFS * C::ACC;
-            const uint32_t idesc = C::FP4 ? (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | (1u << 23) | ((256u >> 7) << 27)
-                                          : (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) |
-                                                ((uint32_t)C::BMN << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-            const uint16_t pair = (uint16_t)(3u << leader);
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        if (warp == 0) {
+            // ---------------- TMA ----------------
+            const int nkb = (p.K + 127) >> 7;
             int it = 0;
-            for (int nt = 0; nt < turns && ok; ++nt) {
-                const int c0 = nt < own ? 0 : s0, c1 = nt < own ? chunks : s1;
-                const int buf = nt % C::BUFS, use = nt / C::BUFS;
-                if (use > 0) ok = warp_all(mb_wait(&tempty[buf], (uint32_t)(use - 1) & 1u, p.status, kWaitDrain));
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t d = tmem + buf * C::ACC;
+            for (int i = 0; i < turns && ok; ++i) {
+                pair_tile(p, i < own ? first + i * step : split, m, n, which);
+                const int c0 = i < own ? 0 : s0, c1 = i < own ? chunks : s1;
+                const int m0 = m * 256 + (int)rank * 128, n0 = C::GATED ? n * 128 : n * 256 + (int)rank * 128;
                 for (int c = c0; c < c1; ++c, ++it) {
-                    const int st = it % C::STAGES;
-                    ok = warp_all(mb_wait(&full[st], (uint32_t)(it / C::STAGES) & 1u, p.status, kWaitStage));
+                    const int st = it % C::STAGES, use = it / C::STAGES;
+                    if (use > 0) ok = warp_all(mb_wait(&empty[st], (uint32_t)(use - 1) & 1u, p.status, kWaitStage));
                     if (!ok) break;
-                    tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t a0 = smem_lo + (uint32_t)(st * (C::STAGE >> 4)), b0 = a0 + (C::HALF >> 4);
-                        if constexpr (C::FP4) {
-                            const uint32_t sf = b0 + (C::HALF >> 4), ts = sf_tmem + (it & 1) * C::SF_COLS;
-                            const int left = p.K - c * C::BK, kbs = left > 128 ? 2 : 1, steps = left >= C::BK ? 4 : (left + 63) >> 6;
-                            for (int kb = 0; kb < kbs; ++kb) {
-                                pair_scales(ts + kb * 4, (sf + kb * 32) << 4);
-                                pair_scales(ts + 8 + kb * 8, (sf + 64 + kb * 32) << 4);
-                                pair_scales(ts + 12 + kb * 8, (sf + 128 + kb * 32) << 4);
-                            }
-                            for (int ks = 0; ks < steps; ++ks)
-                                pair_mma4(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc | ((uint32_t)(ks & 1) << 30) | ((uint32_t)(ks & 1) << 5),
-                                          ts + (ks >> 1) * 4, ts + 8 + (ks >> 1) * 8, c > c0 || ks > 0);
+                        uint8_t *sa = smem + st * C::STAGE, *sb = sa + C::HALF;
+                        const int pass = c >= kch, kc = pass ? c - kch : c;
+                        const uint32_t bar = in_cta(s32(&full[st]), leader);
+                        if (rank == 0) mb_expect_tx(&full[st], 2u * C::STAGE);
+                        const CUtensorMap *ma = &p.a[pass | which], *mb = &p.b[C::GATED ? (int)rank : pass];
+                        if constexpr (C::AMN) {
+                            pair_load_2d(sa, ma, m0, kc * 64, bar);
+                            pair_load_2d(sa + 8192, ma, m0 + 64, kc * 64, bar);
                         } else {
-#pragma unroll
-                            for (int ks = 0; ks < 4; ++ks)
-                                pair_mma16(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc, c > c0 || ks > 0);
+                            pair_load_2d(sa, ma, kc * (C::FP4 ? 128 : 64), m0, bar);
                         }
-                        pair_commit(&empty[st], pair);
-                        if (c == c1 - 1) pair_commit(&tfull[buf], pair);
+                        if constexpr (C::BMN) {
+                            pair_load_2d(sb, mb, n0, kc * 64, bar);
+                            pair_load_2d(sb + 8192, mb, n0 + 64, kc * 64, bar);
+                        } else {
+                            pair_load_2d(sb, mb, kc * (C::FP4 ? 128 : 64), n0, bar);
+                        }
+                        if constexpr (C::FP4) {
+                            uint8_t* sf = sb + C::HALF;
+                            pair_load_2d(sf, &p.sa, 0, (m0 >> 7) * nkb + 2 * kc, bar);
+                            pair_load_2d(sf + 1024, &p.sb[0], 0, (C::GATED ? n : 2 * n) * nkb + 2 * kc, bar);
+                            pair_load_2d(sf + 2048, &p.sb[C::GATED], 0, (C::GATED ? n : 2 * n + 1) * nkb + 2 * kc, bar);
+                        }
                     }
                     __syncwarp();
                 }
             }
+            if (!ok && rank == 0)  // copies in flight, of both CTAs, end before their shared memory is given up
+                for (int i = max(0, it - C::STAGES); i < it; ++i) mb_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
+        } else if (warp == 1) {
+            // ---------------- MMA issue: the leader's thread for both ----------------
+            if (rank == 0) {
+                const uint32_t smem_lo = (s32(smem) & 0x3FFFFu) >> 4;  // in a cluster an address has its CTA's rank above
+                constexpr uint32_t LA = (C::AMN ? (8192u >> 4) : 1u) << 16, LB = (C::BMN ? (8192u >> 4) : 1u) << 16;
+                constexpr uint32_t KA = C::AMN ? 128 : 2, KB = C::BMN ? 128 : 2;
+                const uint32_t sf_tmem = tmem + C::BUFS * C::ACC;
+                const uint32_t idesc = C::FP4 ? (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | (1u << 23) | ((256u >> 7) << 27)
+                                              : (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) |
+                                                    ((uint32_t)C::BMN << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+                const uint16_t pair = (uint16_t)(3u << leader);
+                int it = 0;
+                for (int nt = 0; nt < turns && ok; ++nt) {
+                    const int c0 = nt < own ? 0 : s0, c1 = nt < own ? chunks : s1;
+                    const int buf = nt % C::BUFS, use = nt / C::BUFS;
+                    if (use > 0) ok = warp_all(mb_wait(&tempty[buf], (uint32_t)(use - 1) & 1u, p.status, kWaitDrain));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + buf * C::ACC;
+                    for (int c = c0; c < c1; ++c, ++it) {
+                        const int st = it % C::STAGES;
+                        ok = warp_all(mb_wait(&full[st], (uint32_t)(it / C::STAGES) & 1u, p.status, kWaitStage));
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t a0 = smem_lo + (uint32_t)(st * (C::STAGE >> 4)), b0 = a0 + (C::HALF >> 4);
+                            if constexpr (C::FP4) {
+                                const uint32_t sf = b0 + (C::HALF >> 4), ts = sf_tmem + (it & 1) * C::SF_COLS;
+                                const int left = p.K - c * C::BK, kbs = left > 128 ? 2 : 1, steps = left >= C::BK ? 4 : (left + 63) >> 6;
+                                for (int kb = 0; kb < kbs; ++kb) {
+                                    pair_scales(ts + kb * 4, (sf + kb * 32) << 4);
+                                    pair_scales(ts + 8 + kb * 8, (sf + 64 + kb * 32) << 4);
+                                    pair_scales(ts + 12 + kb * 8, (sf + 128 + kb * 32) << 4);
+                                }
+                                for (int ks = 0; ks < steps; ++ks)
+                                    pair_mma4(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc | ((uint32_t)(ks & 1) << 30) | ((uint32_t)(ks & 1) << 5),
+                                              ts + (ks >> 1) * 4, ts + 8 + (ks >> 1) * 8, c > c0 || ks > 0);
+                            } else {
+#pragma unroll
+                                for (int ks = 0; ks < 4; ++ks)
+                                    pair_mma16(d, desc_of(a0 + ks * KA | LA), desc_of(b0 + ks * KB | LB), idesc, c > c0 || ks > 0);
+                            }
+                            pair_commit(&empty[st], pair);
+                            if (c == c1 - 1) pair_commit(&tfull[buf], pair);
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
         }
+        __syncwarp();
+        if (shares) cluster_sync();  // the shares are written
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
         // ---------------- results ----------------
-        const int quad = warp & 3, half = (warp - 2) >> 2;
-        uint8_t* buf_s = staging + (warp - 2) * C::BOXES * 4096;
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        uint8_t* buf_s = staging + (warp - 4) * C::BOXES * 4096;
         for (int nt = 0; nt < turns && ok; ++nt) {
             const int buf = nt % C::BUFS, use = nt / C::BUFS;
+            // Where to is worked out before the wait: with one accumulator the next tile's MMAs wait for what is between it and the arrival.
+            const uint32_t ta = tmem + buf * C::ACC + ((uint32_t)(quad * 32) << 16), drained = in_cta(s32(&tempty[buf]), leader);
+            pair_tile(p, nt < own ? first + nt * step : split, m, n, which);
+            const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
             ok = warp_all(mb_wait(&tfull[buf], (uint32_t)use & 1u, p.status, kWaitAcc));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t ta = tmem + buf * C::ACC + ((uint32_t)(quad * 32) << 16);
+            float v[4][32];
+            if constexpr (C::BUFS == 1) {
+                if (nt < own) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(ta + (C::GATED ? (c & 2 ? 128 : 0) + half * 64 + 32 * (c & 1) : half * 128 + 32 * c), v[c]);
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) remote_arrive(drained);
+                }
+            }
             if (nt == own) {  // the ring is empty: every copy has landed and been read
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    tmem_ld32(ta + half * 128 + 32 * c, v);
+                    tmem_ld32(ta + half * 128 + 32 * c, v[0]);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<float4*>(smem + share_at(quad * 32 + lane, half * 32 + c * 8 + i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        *reinterpret_cast<float4*>(smem + share_at(quad * 32 + lane, half * 32 + c * 8 + i)) =
+                            make_float4(v[0][4 * i], v[0][4 * i + 1], v[0][4 * i + 2], v[0][4 * i + 3]);
                 }
                 break;
             }
-            pair_tile(p, first + nt * step, m, n, which);
-            const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
-            const uint32_t drained = in_cta(s32(&tempty[buf]), leader);
             switch (p.out_type) {
-                case T_F16: results<C, T_F16>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
-                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
-                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, ta, buf_s, lane, drained); break;
-                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, ta, buf_s, lane, drained);
+                case T_F16: results<C, T_F16>(p, which, row0, n0, half, ta, buf_s, lane, drained, v); break;
+                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, ta, buf_s, lane, drained, v); break;
+                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, ta, buf_s, lane, drained, v); break;
+                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, ta, buf_s, lane, drained, v);
             }
         }
-    }
-    __syncwarp();
-    if (shares) {  // the whole cluster
-        cluster_sync();
-        if (warp >= 2) {
-            const int quad = warp & 3, half = (warp - 2) >> 2, unit = (int)part + half * p.parts;
-            uint8_t* buf_s = staging + (warp - 2) * C::BOXES * 4096;
+        __syncwarp();
+        if (shares) {  // the whole cluster: those of the other warps wait below
+            cluster_sync();
+            const int unit = (int)part + half * p.parts;
             pair_tile(p, split, m, n, which);
             const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
             if (unit < C::NOUT / 64) {
@@ -488,8 +498,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) pair_kernel(const __grid_constant
                 }
             }
         }
+        if (lane == 0) store_done();
     }
-    if (warp >= 2 && lane == 0) store_done();
+    __syncwarp();
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // nobody's shared or tensor memory goes while the other may still use it
@@ -515,7 +526,7 @@ template <class C>
 cudaLaunchConfig_t pair_config(dnb_ctx* c, cudaLaunchAttribute (&at)[2], unsigned grid, int parts) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(NTHREADS);
+    cfg.blockDim = dim3(PAIR_THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = c->stream;
     at[0].id = cudaLaunchAttributeClusterDimension;
