@@ -13,6 +13,8 @@
 // rows do not start or end at multiples of 16 bytes, in whole rows by plain stores).  16 bits: two accumulators; 4 bits, where the scales take the
 // room: one, drained to registers at once so that the next tile's MMAs need not wait for the stores.
 #pragma once
+#include <type_traits>
+
 #include "dense_tc.cuh"
 
 namespace dnb {
@@ -70,16 +72,14 @@ __device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, 
 }
 __device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int MORE>
 __device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(MORE) : "memory"); }
 __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// Says that tensor memory has been read (tcgen05.wait::ld and the fence are before it): nothing else has to be visible, and a release at the cluster's
-// scope would wait 1,300 cycles for the stores of the last tile.
-__device__ __forceinline__ void remote_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
+// Says that tensor memory has been read (tcgen05's wait and fence stand before it).  Released at the cluster's scope it would wait 1,300 cycles for
+// the stores of the last tile, which nobody has to see.
+__device__ __forceinline__ void remote_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void pair_commit(uint64_t* bar, uint16_t pair) {  // the barrier of both CTAs
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(bar)), "h"(pair) : "memory");
 }
@@ -157,23 +157,23 @@ __device__ __forceinline__ void chunk_end(const CUtensorMap* map, bool tma, void
     if (tma) {
         fence_async_smem();
         __syncwarp();
-        if (lane == 0 && row0 < M && col0 < N) store_2d(map, col0, row0, s32(buf));
+        if (lane == 0) {
+            if (row0 < M && col0 < N) store_2d(map, col0, row0, s32(buf));
+            store_commit();  // a group for each box, whether or not it has anything to store: they are counted
+        }
         return;
     }
     __syncwarp();
     const int rows = min(32, M - row0);
     constexpr int SIZE = OUT == T_F32 ? 4 : 2;
-#pragma unroll 1
-    for (int r = 0; r < rows; ++r) {
+    using W = typename std::conditional<OUT == T_F32, float, uint16_t>::type;
 #pragma unroll
-        for (int i = 0; i < 4 / SIZE; ++i) {
-            const int c = 32 * i + lane;
-            if (col0 + c >= N) continue;
-            const uint8_t* src = buf + r * 128 + (((c * SIZE >> 4) ^ (r & 7)) << 4) + (c * SIZE & 15);
-            const size_t at = (size_t)(row0 + r) * ldo + col0 + c;
-            if constexpr (OUT == T_F32) reinterpret_cast<float*>(out)[at] = *reinterpret_cast<const float*>(src);
-            else reinterpret_cast<uint16_t*>(out)[at] = *reinterpret_cast<const uint16_t*>(src);
-        }
+    for (int i = 0; i < 4 / SIZE; ++i) {
+        const int c = 32 * i + lane;
+        if (col0 + c >= N) break;
+        W* to = reinterpret_cast<W*>(out) + (size_t)row0 * ldo + col0 + c;
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) to[r * ldo] = *reinterpret_cast<const W*>(buf + r * 128 + (((c * SIZE >> 4) ^ (r & 7)) << 4) + (c * SIZE & 15));
     }
     __syncwarp();
 }
@@ -229,32 +229,15 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
     }
 }
 
-// This thread's part of a tile, 128 columns (gated: 64 of g and of u).  v: drained from tensor memory already, where there is one accumulator.
+// This thread's part of a tile, 128 columns (gated: 64 of g and of u), in registers: every element by a constant index, so the chunks are unrolled.
 template <class C, int OUT>
-__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint32_t ta, uint8_t*& buf, int lane, uint32_t drained, float (&v)[4][32]) {
+__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint8_t*& buf, int lane, float (&v)[4][32]) {
     constexpr int CHUNKS = C::GATED ? 2 : 4;
-    const int at = half * 32 * CHUNKS;
     const ActForm act = act_form(p.act);
     uint32_t first[16];
-    if constexpr (C::BUFS == 1) {
-        // every element by a constant index, so the chunks are unrolled
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, v[c], v[C::GATED ? 2 + c : c], buf, lane, first);
-    } else {
-        // one chunk's code: unrolled, it would not fit the instruction cache
-#pragma unroll 1
-        for (int c = 0; c < CHUNKS; ++c) {
-            tmem_ld32(ta + at + 32 * c, v[0]);
-            if constexpr (C::GATED) tmem_ld32(ta + 128 + at + 32 * c, v[1]);
-            tmem_ld_wait();
-            if (c == CHUNKS - 1) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) remote_arrive(drained);
-            }
-            chunk_of<C, OUT>(p, act, which, c, row0, n0 + at + 32 * c, v[0], v[1], buf, lane, first);
-        }
-    }
+    for (int c = 0; c < CHUNKS; ++c)
+        chunk_of<C, OUT>(p, act, which, c, row0, n0 + 32 * (half * CHUNKS + c), v[c], v[C::GATED ? 2 + c : c], buf, lane, first);
 }
 
 // A split tile.  This CTA's sums in the ring's memory, four columns of all rows after another: what a warp reads of another CTA's is 512 bytes in a
@@ -446,7 +429,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
         uint8_t* buf_s = staging + (warp - 4) * C::BOXES * 4096;
         for (int nt = 0; nt < turns && ok; ++nt) {
             const int buf = nt % C::BUFS, use = nt / C::BUFS;
-            // Where to is worked out before the wait: with one accumulator the next tile's MMAs wait for what is between it and the arrival.
+            // Where to is worked out before the wait: with one accumulator the next tile's MMAs wait for what is between it and the arrival.  All of a
+            // thread's columns are read at once, with two accumulators, too: 32 at a time, each waited for, took 2.6 times as long a tile.
             const uint32_t ta = tmem + buf * C::ACC + ((uint32_t)(quad * 32) << 16), drained = in_cta(s32(&tempty[buf]), leader);
             pair_tile(p, nt < own ? first + nt * step : split, m, n, which);
             const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
@@ -454,15 +438,13 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
             if (!ok) break;
             tc_fence_after();
             float v[4][32];
-            if constexpr (C::BUFS == 1) {
-                if (nt < own) {
+            if (nt < own) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(ta + (C::GATED ? (c & 2 ? 128 : 0) + half * 64 + 32 * (c & 1) : half * 128 + 32 * c), v[c]);
-                    tmem_ld_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) remote_arrive(drained);
-                }
+                for (int c = 0; c < 4; ++c) tmem_ld32(ta + (C::GATED ? (c & 2 ? 128 : 0) + half * 64 + 32 * (c & 1) : half * 128 + 32 * c), v[c]);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) remote_arrive(drained);
             }
             if (nt == own) {  // the ring is empty: every copy has landed and been read
 #pragma unroll 1
@@ -477,10 +459,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
                 break;
             }
             switch (p.out_type) {
-                case T_F16: results<C, T_F16>(p, which, row0, n0, half, ta, buf_s, lane, drained, v); break;
-                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, ta, buf_s, lane, drained, v); break;
-                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, ta, buf_s, lane, drained, v); break;
-                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, ta, buf_s, lane, drained, v);
+                case T_F16: results<C, T_F16>(p, which, row0, n0, half, buf_s, lane, v); break;
+                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, buf_s, lane, v); break;
+                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, buf_s, lane, v); break;
+                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, buf_s, lane, v);
             }
         }
         __syncwarp();

@@ -104,6 +104,28 @@ def test_both_directions(cu, ctx, act, name, nt, k, n):
         assert bool((b.out[:, n:] == 7).all()) and bool((b.dx[:, k:] == 7).all())
 
 
+@pytest.mark.parametrize("nt,k,n", [(77, 2056, 5640), (3000, 72, 2056), (8, 4096, 4096), (2000, 2048, 136)])
+def test_many_tiles(cu, ctx, nt, k, n):
+    """Several tiles for every SM, with next to nothing between them: sums of the kernel's own 16-bit operands, every time the same bits."""
+    b = Block(cu, "silu", "bf16", nt, k, n)
+    first = None
+    for _ in range(4):
+        for t in (b.out, b.dx, b.dg, b.du):
+            t.fill_(7)
+        assert b.forward(ctx) and b.backward(ctx)
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (b.out, b.pre, b.dx, b.dg, b.du)]
+        first = first or got
+        assert all(torch.equal(p, q) for p, q in zip(got, first))
+    x, wg, wu, _ = (v.cuda() for v in b.wide())
+    dg, du, half = b.dpre[0].double(), b.dpre[1].double(), dh.half_step(b.t)
+    for got, want, off in ((b.pre[0], x @ wg.T, dh.sum_error(k, x.abs() @ wg.abs().T)), (b.pre[1], x @ wu.T, dh.sum_error(k, x.abs() @ wu.abs().T)),
+                           (b.dg, dg.T @ x, dh.sum_error(nt, dg.abs().T @ x.abs())), (b.du, du.T @ x, dh.sum_error(nt, du.abs().T @ x.abs())),
+                           (b.dx, dg @ wg + du @ wu, dh.sum_error(2 * n, dg.abs() @ wg.abs() + du.abs() @ wu.abs()))):
+        off = off + (half * (want.abs() + off) if got.dtype is b.t else 0)
+        assert int(((got.double() - want).abs() > off + dh.floor_of(b.t)).sum()) == 0
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gradients_against_differences(cu, ctx, act):
     """Along random directions: (f(p + h d) - f(p - h d)) / 2 h in 64 bits against the kernel's gradients."""

@@ -166,6 +166,47 @@ def test_product(cu, ctx, nt, k, n, name):
     check(got, want, dh.sum_error(k, size) + dh.half_step(TYPES[name]) * want.abs() + dh.floor_of(TYPES[name]))
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("nt,k,n", [(3000, 64, 4100), (5000, 256, 2048), (2600, 544, 5003), (90, 96, 70000)])
+def test_product_of_many_tiles(cu, ctx, nt, k, n, name):
+    """Several tiles for every SM, with next to nothing between them: each tile's results are its own, every time."""
+    gen = torch.Generator().manual_seed(nt + k + n)
+    x, w = dh.random_codes(gen, nt, k, 120, 125), dh.random_codes(gen, n, k, 120, 125)
+    (xc, xs), (wc, ws) = dh.pack(*x), dh.pack(*w)
+    vx, vw = dh.values(*x).cuda(), dh.values(*w).cuda()
+    want = vx @ vw.T
+    off = dh.sum_error(k, vx.abs() @ vw.abs().T) + dh.half_step(TYPES[name]) * want.abs() + dh.floor_of(TYPES[name])
+    for _ in range(4):
+        out = torch.full((nt, n), 77.0, dtype=TYPES[name], device="cuda")
+        assert ctx.mx4_gemm_dev(xc.data_ptr(), xs.data_ptr(), wc.data_ptr(), ws.data_ptr(), nt, k, n, ids(cu)[name], out.data_ptr())
+        torch.cuda.synchronize()
+        assert int(((out.double() - want).abs() > off).sum()) == 0
+
+
+@pytest.mark.parametrize("nt,k,n", [(3000, 64, 4128), (2600, 256, 4096)])
+def test_gated_of_many_tiles(cu, ctx, nt, k, n):
+    gen = torch.Generator().manual_seed(nt + k + n)
+    x, g, u = dh.random_codes(gen, nt, k, 124, 128), dh.random_codes(gen, n, k, 119, 123), dh.random_codes(gen, n, k, 119, 123)
+    (xc, xs), (gc, gs), (uc, us) = (dh.pack(*m) for m in (x, g, u))
+    vx, vg, vu = (dh.values(*m).cuda() for m in (x, g, u))
+    wg, wu = vx @ vg.T, vx @ vu.T
+    want = dh.act("silu", wg) * wu
+    off_g, off_u = dh.sum_error(k, vx.abs() @ vg.abs().T), dh.sum_error(k, vx.abs() @ vu.abs().T)
+    off = (dh.SLOPE * off_g + 2.0 ** -20 * wg.abs()) * (wu.abs() + off_u) + dh.act("silu", wg).abs() * off_u
+    ptrs = [t.data_ptr() for t in (xc, xs, gc, gs, uc, us)]
+    for _ in range(4):
+        out = torch.full((nt, n), 77.0, device="cuda")
+        assert ctx.mx4_gated_dev(cu.ACT_SILU, *ptrs, nt, k, n, cu.F32, out.data_ptr())
+        codes, scales = buffers(cu, nt, n)
+        assert ctx.mx4_gated_dev(cu.ACT_SILU, *ptrs, nt, k, n, cu.MXFP4, codes.data_ptr(), scales.data_ptr())
+        again, again_s = quantised(cu, ctx, out, "f32")
+        torch.cuda.synchronize()
+        assert int(((out.double() - want).abs() > off + dh.half_step(torch.float32) * want.abs()).sum()) == 0
+        assert torch.equal(codes, again)
+        code, e = dh.unpack(codes, scales, nt, n)
+        assert torch.equal(e, dh.unpack(again, again_s, nt, n)[1])
+
+
 def test_product_nan_and_far_scales(cu, ctx):
     """A NaN scale makes its row's results NaN and no other's; scales at both ends of their range meet."""
     gen = torch.Generator().manual_seed(8)
