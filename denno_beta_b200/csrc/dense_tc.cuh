@@ -125,6 +125,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  "r"(s32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -186,56 +187,87 @@ __device__ __forceinline__ void tile_out(const Params& p, int tile, uint32_t tac
     }
 }
 
-// The sum of a column's shares, in rank order: a warp a column, four neighbouring features a lane, all shares asked for at once.
+// Four neighbouring results, of which `left` exist; whole: 8- or 16-byte stores are aligned.
+template <int OUT>
+__device__ __forceinline__ void put4(void* out, size_t at, const float (&o)[4], int left, bool whole) {
+    if (whole && left >= 4) {
+        if constexpr (OUT == T_F32) {
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = make_float4(o[0], o[1], o[2], o[3]);
+        } else {
+            uint16_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put<OUT>(h, i, o[i]);
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < left) put<OUT>(out, at + i, o[i]);
+}
+// The sums of columns' shares, in rank order: a warp two columns at a time, four neighbouring features a lane, all shares asked for at once.
 template <class C, int OUT>
 __device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t red, uint32_t rank, int warp, int lane) {
-    const int m = tile * TM + 4 * lane;
+    const int m = tile * TM + 4 * lane, left = p.M - m;
     const ActForm act = act_form(p.act);
+    const bool whole = ((p.ldo | (reinterpret_cast<uintptr_t>(p.out) / (OUT == T_F32 ? 4 : 2))) & 3) == 0;
+    const int step = EPI_WARPS * p.splits;
 #pragma unroll 1
-    for (int c = (int)rank + p.splits * warp; c < p.N; c += EPI_WARPS * p.splits) {
-        float4 v[C::NA][8];
-#pragma unroll
-        for (int a = 0; a < C::NA; ++a)
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (r < p.splits) v[a][r] = peer_floats(red + 4u * (uint32_t)((a * C::BN + c) * TM + 4 * lane), r);
-        float4 s[C::NA];
-#pragma unroll
-        for (int a = 0; a < C::NA; ++a) {
-            s[a] = v[a][0];
-#pragma unroll
-            for (int r = 1; r < 8; ++r)
-                if (r < p.splits) {
-                    s[a].x += v[a][r].x; s[a].y += v[a][r].y; s[a].z += v[a][r].z; s[a].w += v[a][r].w;
-                }
-        }
-        float o[4] = {s[0].x, s[0].y, s[0].z, s[0].w};
-        if constexpr (C::NA == 2) {
-            const float u[4] = {s[1].x, s[1].y, s[1].z, s[1].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (p.pre && m + i < p.M) {
-                    p.pre[(size_t)c * p.M + m + i] = o[i];
-                    p.pre[((size_t)p.N + c) * p.M + m + i] = u[i];
-                }
-                o[i] = act_of(act, o[i]) * u[i];
-            }
-        }
-        if constexpr (OUT == T_MXFP4) {  // a block is eight lanes
-            uint32_t mx = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(o[i]) & 0x7fffffffu);
-#pragma unroll
-            for (int d = 1; d < 8; d <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const uint32_t e = scale_byte(mx);
-            const float by = scale_inverse(e);
-            const uint32_t code = e2m1_pair(o[0] * by, o[1] * by) | e2m1_pair(o[2] * by, o[3] * by) << 8;
-            if (m < p.M) *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.out) + ((size_t)c * p.M + m) / 2) = (uint16_t)(e == 255 ? 0u : code);
-            if ((lane & 7) == 0) p.out_scales[scale_at(c, m >> 5, (p.M + 127) >> 7)] = (uint8_t)(m < p.M ? e : 0u);
-        } else {
+    for (int c0 = (int)rank + p.splits * warp; c0 < p.N; c0 += 2 * step) {
+        float4 s[2][C::NA];
+        for (int r = 0; r < p.splits; r += 4) {
+            float4 v[2][C::NA][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (m + i < p.M) put<OUT>(p.out, (size_t)c * p.ldo + m + i, o[i]);
+                if (r + i < p.splits) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int a = 0; a < C::NA; ++a)  // a second column beyond the last reads where the ring was
+                            v[j][a][i] = peer_floats(red + 4u * (uint32_t)((a * C::BN + min(c0 + j * step, C::BN - 1)) * TM + 4 * lane), r + i);
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r + i < p.splits) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int a = 0; a < C::NA; ++a) {
+                            float4& d = s[j][a];
+                            const float4 t = v[j][a][i];
+                            if (r + i == 0) d = t;
+                            else d.x += t.x, d.y += t.y, d.z += t.z, d.w += t.w;
+                        }
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int c = c0 + j * step;
+            if (c >= p.N) break;
+            float o[4] = {s[j][0].x, s[j][0].y, s[j][0].z, s[j][0].w};
+            if constexpr (C::NA == 2) {
+                const float u[4] = {s[j][1].x, s[j][1].y, s[j][1].z, s[j][1].w};
+                if (p.pre) {  // M is a multiple of eight
+                    put4<T_F32>(p.pre, (size_t)c * p.M + m, o, left, true);
+                    put4<T_F32>(p.pre, ((size_t)p.N + c) * p.M + m, u, left, true);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = act_of(act, o[i]) * u[i];
+            }
+            if constexpr (OUT == T_MXFP4) {  // a block is eight lanes
+                uint32_t mx = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(o[i]) & 0x7fffffffu);
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                const uint32_t e = scale_byte(mx);
+                const float by = scale_inverse(e);
+                const uint32_t code = e2m1_pair(o[0] * by, o[1] * by) | e2m1_pair(o[2] * by, o[3] * by) << 8;
+                if (left > 0) *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.out) + ((size_t)c * p.M + m) / 2) = (uint16_t)(e == 255 ? 0u : code);
+                if ((lane & 7) == 0) p.out_scales[scale_at(c, m >> 5, (p.M + 127) >> 7)] = (uint8_t)(left > 0 ? e : 0u);
+            } else {
+                put4<OUT>(p.out, (size_t)c * p.ldo + m, o, left, whole);
+            }
         }
     }
 }
@@ -262,6 +294,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
         }
         fence_mbarrier_init();
     }
+    if (warp == 0 && lane < 4) prefetch_map(lane < 2 ? &p.a[lane & (C::NA == 2 ? 1 : p.passes - 1)] : &p.b[lane & (p.passes - 1)]);
     if (warp == 1) tmem_alloc<C::COLS>(tmem_slot);
     tc_fence_before();
     __syncthreads();
@@ -398,6 +431,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
                 float* red = reinterpret_cast<float*>(smem);
                 const uint32_t ta = tacc + ((uint32_t)(quad * 32) << 16);
                 for (int g = half; g < C::ACC / 16; g += 2) {
+                    if (g * 16 % C::BN >= p.N) continue;
                     uint32_t v[16];
                     tmem_ld16(ta + 16 * g, v);
                     tmem_ld_wait();

@@ -12,142 +12,248 @@ using namespace dt;
 using dt::Cfg;
 using dt::Params;
 
-// 16 threads a unit of 128 elements of a row (a scale tile's width), 8 elements a thread; a block of 32 is four neighbouring lanes.
-constexpr int UNIT_THREADS = 16, THREADS = 256, UNITS = THREADS / UNIT_THREADS;
+// A thread takes 8 elements of the rows r, r + 32, r + 64 and r + 96 of a tile of scales, 16 threads (half a warp) its 128 columns: four independent
+// 16- or 32-byte loads in flight a thread, and the 16 bytes of scales that these rows have next to each other are one store.  A block of 32 is four
+// neighbouring lanes.  Bound by memory: 14018 x 4096, fp32 to 4 bits 40 us (6.5 TB/s), bf16 29 (5.0) and back 29 (a row a thread at a time, 64-bit
+// divisions and a branch at each load, which waited for it: 47 and 37).
+constexpr int THREADS = 256, UNITS = THREADS / 16;
+
+// Where a thread is: unit u = folded row * nkb + kb, a folded row being 32 * tile + r.  Advanced without a division.
+struct Walk {
+    size_t u, units, row;  // row: the first of the four
+    int kb, nkb, dkb;
+    size_t dq, q;
+    __device__ Walk(size_t folded, int nkb_) : units(folded * nkb_), nkb(nkb_) {
+        u = (size_t)blockIdx.x * UNITS + (threadIdx.x >> 4);
+        const size_t step = (size_t)gridDim.x * UNITS;
+        if (units >> 31) {
+            q = u / nkb; kb = (int)(u - q * nkb); dq = step / nkb; dkb = (int)(step - dq * nkb);
+        } else {
+            const uint32_t qs = (uint32_t)u / (uint32_t)nkb, ds = (uint32_t)step / (uint32_t)nkb;
+            q = qs; kb = (int)((uint32_t)u - qs * nkb); dq = ds; dkb = (int)((uint32_t)step - ds * nkb);
+        }
+        place();
+    }
+    __device__ void place() { row = (q >> 5) * 128 + (q & 31); }
+    __device__ bool warp_in() const { return u - ((threadIdx.x >> 4) & 1) < units; }  // the first of the warp's two units
+    __device__ void next() {
+        u += (size_t)gridDim.x * UNITS;
+        q += dq;
+        kb += dkb;
+        if (kb >= nkb) kb -= nkb, ++q;
+        place();
+    }
+};
+static size_t folded_rows(int rows) { return (size_t)(rows / 128) * 32 + (rows % 128 < 32 ? rows % 128 : 32); }
 
 template <int T> struct Num { using type = float; };
 template <> struct Num<T_F16> { using type = __half; };
 template <> struct Num<T_BF16> { using type = __nv_bfloat16; };
 
-// Eight elements from `at`; whole says that the pointer is 16-byte aligned (rows may start anywhere).
-template <int T>
-__device__ __forceinline__ void load8(const void* x, size_t at, bool whole, float (&v)[8]) {
-    if constexpr (T == T_F32) {
-        const float* s = reinterpret_cast<const float*>(x) + at;
-        if (whole) {
-            const float4 a = reinterpret_cast<const float4*>(s)[0], b = reinterpret_cast<const float4*>(s)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
+// Eight elements as loaded (rows may start anywhere; WHOLE: at multiples of 16 bytes), and as numbers.
+template <int T> struct Raw { uint32_t w[T == T_F32 ? 8 : 4]; };
+template <int T, bool WHOLE>
+__device__ __forceinline__ Raw<T> load8(const void* x, size_t at) {
+    Raw<T> r;
+    if constexpr (WHOLE) {
+        const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const typename Num<T>::type*>(x) + at);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = s[i];
+        for (int i = 0; i < (T == T_F32 ? 2 : 1); ++i) {
+            const uint4 v = s[i];
+            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
         }
+    } else if constexpr (T == T_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.w[i] = reinterpret_cast<const uint32_t*>(x)[at + i];
     } else {
-        using N = typename Num<T>::type;
-        N s[8];
-        const N* src = reinterpret_cast<const N*>(x) + at;
-        if (whole) {
-            *reinterpret_cast<uint4*>(s) = *reinterpret_cast<const uint4*>(src);
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(x) + at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = s[2 * i] | (uint32_t)s[2 * i + 1] << 16;
+    }
+    return r;
+}
+template <int T>
+__device__ __forceinline__ void numbers(const Raw<T>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (T == T_F32) {
+            v[2 * i] = __uint_as_float(r.w[2 * i]);
+            v[2 * i + 1] = __uint_as_float(r.w[2 * i + 1]);
+        } else if constexpr (T == T_BF16) {
+            v[2 * i] = __uint_as_float(r.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = src[i];
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)s[i];
     }
 }
-
-// Units u = row * nkb + kb.
+// Bits, as fp32, of the largest magnitudes of four rows' blocks (four neighbouring lanes).  16-bit magnitudes are compared two rows a word.
 template <int T>
-__global__ void __launch_bounds__(THREADS)
-quantize_kernel(const void* __restrict__ x, size_t ldx, bool whole, size_t units, int k, int nkb, uint8_t* __restrict__ codes,
-                uint8_t* __restrict__ scales) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & (UNIT_THREADS - 1);
-    // whole warps stay in the loop: a warp's two units are neighbours
-    for (size_t u0 = (size_t)blockIdx.x * UNITS + (threadIdx.x >> 5) * 2; u0 < units; u0 += (size_t)gridDim.x * UNITS) {
-        const size_t u = u0 + ((threadIdx.x >> 4) & 1);
-        const size_t row = u / nkb;
-        const int kb = (int)(u - row * nkb), at = kb * 128 + lane * 8;
-        const bool in = u < units && at < k;
-        float v[8] = {};
-        if (in) load8<T>(x, row * ldx + at, whole, v);
-        uint32_t mx = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const uint32_t e = scale_byte(mx);
-        const uint32_t code = e2m1_eight(v, scale_inverse(e));
-        if (in) *reinterpret_cast<uint32_t*>(codes + (row * k + at) / 2) = e == 255 ? 0u : code;
-        uint32_t s = in ? e << (8 * (lane >> 2)) : 0u;
-        s |= __shfl_xor_sync(0xffffffffu, s, 4);
-        s |= __shfl_xor_sync(0xffffffffu, s, 8);
-        if (lane == 0 && u < units) *reinterpret_cast<uint32_t*>(scales + scale_at(row, 4 * kb, nkb)) = s;
-    }
-}
-
-// Blocks of a GGUF file: the scale's byte, then 16 bytes with elements 0 to 15 in their low halves and 16 to 31 in the high ones.
-__global__ void __launch_bounds__(THREADS)
-relay_kernel(const uint8_t* __restrict__ blocks, size_t ldx, size_t units, int k, int nkb, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & (UNIT_THREADS - 1);
-    for (size_t u0 = (size_t)blockIdx.x * UNITS + (threadIdx.x >> 5) * 2; u0 < units; u0 += (size_t)gridDim.x * UNITS) {
-        const size_t u = u0 + ((threadIdx.x >> 4) & 1);
-        const size_t row = u / nkb;
-        const int kb = (int)(u - row * nkb), at = kb * 128 + lane * 8;
-        const bool in = u < units && at < k;
-        uint32_t code = 0, e = 0;
-        if (in) {
-            const uint8_t* b = blocks + (row * ldx + at) / 32 * 17;
-            const int first = at & 15, high = at & 16 ? 4 : 0;
-            e = b[0];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) code |= (uint32_t)((b[1 + first + i] >> high) & 15) << (4 * i);
-            *reinterpret_cast<uint32_t*>(codes + (row * k + at) / 2) = code;
-        }
-        uint32_t s = e << (8 * (lane >> 2));
-        s |= __shfl_xor_sync(0xffffffffu, s, 4);
-        s |= __shfl_xor_sync(0xffffffffu, s, 8);
-        if (lane == 0 && u < units) *reinterpret_cast<uint32_t*>(scales + scale_at(row, 4 * kb, nkb)) = s;
-    }
-}
-
-template <int T>
-__global__ void __launch_bounds__(THREADS)
-dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, size_t units, int k, int nkb, void* __restrict__ out, size_t ldo,
-                  bool whole) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & (UNIT_THREADS - 1);
-    for (size_t u = (size_t)blockIdx.x * UNITS + (threadIdx.x >> 4); u < units; u += (size_t)gridDim.x * UNITS) {
-        const size_t row = u / nkb;
-        const int kb = (int)(u - row * nkb), at = kb * 128 + lane * 8;
-        if (at >= k) continue;
-        const uint32_t code = *reinterpret_cast<const uint32_t*>(codes + (row * k + at) / 2);
-        const uint32_t e = scales[scale_at(row, at >> 5, nkb)];
-        const float s = __uint_as_float(e == 255 ? 0x7fc00000u : e ? e << 23 : 0x00400000u);
-        float v[8];
+__device__ __forceinline__ void block_max(const Raw<T> (&r)[4], uint32_t (&mx)[4]) {
+    if constexpr (T == T_F32) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t h2;
-            asm("{\n\t.reg .b8 b, z;\n\tmov.b16 {b, z}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h2) : "h"((uint16_t)((code >> (8 * i)) & 0xff)));
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-            v[2 * i] = f.x * s;
-            v[2 * i + 1] = f.y * s;
-        }
-        const size_t o = row * ldo + at;
-        if constexpr (T == T_F32) {
-            float* d = reinterpret_cast<float*>(out) + o;
-            if (whole) {
-                reinterpret_cast<float4*>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
+            mx[i] = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = v[i];
+            for (int j = 0; j < 8; ++j) mx[i] = max(mx[i], r[i].w[j] & 0x7fffffffu);
+            mx[i] = max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+            mx[i] = max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        }
+    } else {
+        uint32_t m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a = __vmaxu2(__vmaxu2(r[i].w[0] & 0x7fff7fffu, r[i].w[1] & 0x7fff7fffu), __vmaxu2(r[i].w[2] & 0x7fff7fffu, r[i].w[3] & 0x7fff7fffu));
+            m[i] = max(a & 0xffffu, a >> 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            uint32_t two = m[i] | m[i + 1] << 16;
+            two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 1));
+            two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 2));
+            if constexpr (T == T_BF16) {
+                mx[i] = two << 16;
+                mx[i + 1] = two & 0xffff0000u;
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+                mx[i] = __float_as_uint(f.x);
+                mx[i + 1] = __float_as_uint(f.y);
+            }
+        }
+    }
+}
+
+// Eight elements as they lie in a GGUF file's blocks: the scale's byte, then 16 bytes with elements 0 to 15 in their low halves and 16 to 31 in the
+// high ones.
+__device__ __forceinline__ void file_piece(const uint8_t* b, int at, uint32_t& code, uint32_t& e) {
+    const int first = at & 15, high = at & 16 ? 4 : 0;
+    e = b[0];
+    code = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code |= (uint32_t)((b[1 + first + i] >> high) & 15) << (4 * i);
+}
+
+template <int T, bool WHOLE>
+__global__ void __launch_bounds__(THREADS)
+quantize_kernel(const void* __restrict__ x, size_t ldx, int rows, size_t folded, int k, int nkb, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 15;
+    const size_t apart = (size_t)16 * k;  // bytes of codes from one of the four rows to the next
+    for (Walk w(folded, nkb); w.warp_in(); w.next()) {
+        const int at = w.kb * 128 + lane * 8;
+        const bool col = w.u < w.units && at < k;
+        const int here = col ? (int)min((size_t)4, ((size_t)rows - w.row + 31) / 32) : 0;  // of the four rows
+        uint32_t code[4], e[4];
+        if constexpr (T == T_MXFP4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                code[i] = e[i] = 0;
+                if (i < here) file_piece(reinterpret_cast<const uint8_t*>(x) + ((w.row + 32 * i) * ldx + at) / 32 * 17, at, code[i], e[i]);
             }
         } else {
-            using N = typename Num<T>::type;
-            N h[8];
+            Raw<T> r[4] = {};
+            const size_t first = w.row * ldx + at;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) put<T>(h, i, v[i]);
-            N* d = reinterpret_cast<N*>(out) + o;
-            if (whole) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(h);
-            else {
+            for (int i = 0; i < 4; ++i)
+                if (i < here) r[i] = load8<T, WHOLE>(x, first + (size_t)(32 * i) * ldx);
+            block_max<T>(r, e);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = h[i];
+            for (int i = 0; i < 4; ++i) {
+                float v[8];
+                numbers<T>(r[i], v);
+                e[i] = scale_byte(e[i]);
+                code[i] = e2m1_eight(v, scale_inverse(e[i]));
+                if (e[i] == 255) code[i] = 0;
+                if (!col) e[i] = 0;
+            }
+        }
+        uint8_t* to = codes + (w.row * k + at) / 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < here) *reinterpret_cast<uint32_t*>(to + i * apart) = code[i];
+        // Four lanes' bytes of four rows to a word a row.
+        const uint32_t b0 = e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, b1 = __shfl_down_sync(0xffffffffu, b0, 4, 16),
+                       b2 = __shfl_down_sync(0xffffffffu, b0, 8, 16), b3 = __shfl_down_sync(0xffffffffu, b0, 12, 16);
+        if (lane == 0 && here > 0) {
+            const uint32_t p = __byte_perm(b0, b1, 0x5140), q = __byte_perm(b2, b3, 0x5140), r = __byte_perm(b0, b1, 0x7362), t = __byte_perm(b2, b3, 0x7362);
+            const uint32_t word[4] = {__byte_perm(p, q, 0x5410), __byte_perm(p, q, 0x7632), __byte_perm(r, t, 0x5410), __byte_perm(r, t, 0x7632)};
+            uint32_t* s = reinterpret_cast<uint32_t*>(scales + scale_at(w.row, 4 * w.kb, nkb));
+            if (here == 4) {
+                *reinterpret_cast<uint4*>(s) = make_uint4(word[0], word[1], word[2], word[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (i < here) s[i] = word[i];
+            }
+        }
+    }
+}
+
+// Four codes (16 bits) as numbers.
+__device__ __forceinline__ void four_values(uint32_t code, float s, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t h2;
+        asm("{\n\t.reg .b8 b, z;\n\tmov.b16 {b, z}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h2) : "h"((uint16_t)((code >> (8 * i)) & 0xff)));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+        v[2 * i] = f.x * s;
+        v[2 * i + 1] = f.y * s;
+    }
+}
+
+// 16 bytes of results a store, neighbouring lanes next to each other: 8 elements a lane, or (F32) 4 of each half of the 128 columns.
+template <int T, bool WHOLE>
+__global__ void __launch_bounds__(THREADS)
+dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, size_t folded, int k, int nkb, void* __restrict__ out, size_t ldo) {
+    pdl_wait();
+    pdl_launch_dependents();
+    using N = typename Num<T>::type;
+    constexpr int EACH = T == T_F32 ? 4 : 8, PIECES = 8 / EACH;
+    const int lane = threadIdx.x & 15;
+    const size_t apart = (size_t)16 * k;
+    for (Walk w(folded, nkb); w.u < w.units; w.next()) {
+        const int here = (int)min((size_t)4, ((size_t)rows - w.row + 31) / 32);
+        uint32_t code[PIECES][4];
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+            const int at = w.kb * 128 + 64 * h + lane * EACH;
+            const uint8_t* from = codes + (w.row * k + at) / 2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i >= here || at >= k) code[h][i] = 0;
+                else if constexpr (T == T_F32) code[h][i] = *reinterpret_cast<const uint16_t*>(from + i * apart);
+                else code[h][i] = *reinterpret_cast<const uint32_t*>(from + i * apart);
+            }
+        }
+        const uint4 s4 = *reinterpret_cast<const uint4*>(scales + scale_at(w.row, 4 * w.kb, nkb));  // rows past the last: read, not used
+        const uint32_t word[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+            const int in = 64 * h + lane * EACH, at = w.kb * 128 + in;
+            N* to = reinterpret_cast<N*>(out) + w.row * ldo + at;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r >= here || at >= k) continue;
+                const uint32_t e = (word[r] >> (8 * (in >> 5))) & 255u;
+                const float s = __uint_as_float(e == 255 ? 0x7fc00000u : e ? e << 23 : 0x00400000u);
+                N* d = to + (size_t)(32 * r) * ldo;
+                alignas(16) N v[EACH];
+#pragma unroll
+                for (int i = 0; i < EACH / 4; ++i) {
+                    float f[4];
+                    four_values(code[h][r] >> (16 * i), s, f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) put<T>(v, 4 * i + j, f[j]);
+                }
+                if constexpr (WHOLE) {
+                    *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) d[i] = v[i];
+                }
             }
         }
     }
@@ -251,17 +357,16 @@ int dnb_mx4_quantize_dev(dnb_ctx* c, int type, const void* x_dev, size_t ldx, in
     if (rows == 0) return DNB_OK;
     DNB_CUDA(cudaSetDevice(c->device));
     const int nkb = (k + 127) / 128;
-    const size_t units = (size_t)rows * nkb;
-    const dim3 grid(grid_of(c, units)), block(THREADS);
+    const size_t folded = folded_rows(rows);
+    const dim3 grid(grid_of(c, folded * nkb)), block(THREADS);
     const bool whole = aligned16(x_dev) && ldx * es % 16 == 0;
     uint8_t *codes = (uint8_t*)codes_dev, *scales = (uint8_t*)scales_dev;
     ProfScope prof_(c, c->stream, "mx4_quantize");
-    switch (type) {
-        case T_F32: DNB_CUDA(launch_k(quantize_kernel<T_F32>, grid, block, 0, c->stream, c->use_pdl, x_dev, ldx, whole, units, k, nkb, codes, scales)); break;
-        case T_F16: DNB_CUDA(launch_k(quantize_kernel<T_F16>, grid, block, 0, c->stream, c->use_pdl, x_dev, ldx, whole, units, k, nkb, codes, scales)); break;
-        case T_BF16: DNB_CUDA(launch_k(quantize_kernel<T_BF16>, grid, block, 0, c->stream, c->use_pdl, x_dev, ldx, whole, units, k, nkb, codes, scales)); break;
-        default: DNB_CUDA(launch_k(relay_kernel, grid, block, 0, c->stream, c->use_pdl, (const uint8_t*)x_dev, ldx, units, k, nkb, codes, scales));
-    }
+#define QUANTIZE(T) (whole ? launch_k(quantize_kernel<T, true>, grid, block, 0, c->stream, c->use_pdl, x_dev, ldx, rows, folded, k, nkb, codes, scales) \
+                           : launch_k(quantize_kernel<T, false>, grid, block, 0, c->stream, c->use_pdl, x_dev, ldx, rows, folded, k, nkb, codes, scales))
+    DNB_CUDA(type == T_F32 ? QUANTIZE(T_F32) : type == T_F16 ? QUANTIZE(T_F16) : type == T_BF16 ? QUANTIZE(T_BF16)
+             : launch_k(quantize_kernel<T_MXFP4, false>, grid, block, 0, c->stream, c->use_pdl, x_dev, ldx, rows, folded, k, nkb, codes, scales));
+#undef QUANTIZE
     c->launches++;
     return DNB_OK;
 }
@@ -282,16 +387,15 @@ int dnb_mx4_dequantize_dev(dnb_ctx* c, const void* codes_dev, const void* scales
     if (rows == 0) return DNB_OK;
     DNB_CUDA(cudaSetDevice(c->device));
     const int nkb = (k + 127) / 128;
-    const size_t units = (size_t)rows * nkb;
-    const dim3 grid(grid_of(c, units)), block(THREADS);
+    const size_t folded = folded_rows(rows);
+    const dim3 grid(grid_of(c, folded * nkb)), block(THREADS);
     const bool whole = aligned16(out_dev) && ldo * es % 16 == 0;
     const uint8_t *codes = (const uint8_t*)codes_dev, *scales = (const uint8_t*)scales_dev;
     ProfScope prof_(c, c->stream, "mx4_dequantize");
-    switch (type) {
-        case T_F32: DNB_CUDA(launch_k(dequantize_kernel<T_F32>, grid, block, 0, c->stream, c->use_pdl, codes, scales, units, k, nkb, out_dev, ldo, whole)); break;
-        case T_F16: DNB_CUDA(launch_k(dequantize_kernel<T_F16>, grid, block, 0, c->stream, c->use_pdl, codes, scales, units, k, nkb, out_dev, ldo, whole)); break;
-        default: DNB_CUDA(launch_k(dequantize_kernel<T_BF16>, grid, block, 0, c->stream, c->use_pdl, codes, scales, units, k, nkb, out_dev, ldo, whole));
-    }
+#define DEQUANTIZE(T) (whole ? launch_k(dequantize_kernel<T, true>, grid, block, 0, c->stream, c->use_pdl, codes, scales, rows, folded, k, nkb, out_dev, ldo) \
+                             : launch_k(dequantize_kernel<T, false>, grid, block, 0, c->stream, c->use_pdl, codes, scales, rows, folded, k, nkb, out_dev, ldo))
+    DNB_CUDA(type == T_F32 ? DEQUANTIZE(T_F32) : type == T_F16 ? DEQUANTIZE(T_F16) : DEQUANTIZE(T_BF16));
+#undef DEQUANTIZE
     c->launches++;
     return DNB_OK;
 }
