@@ -134,6 +134,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same for reads alone: does not wait for this thread's stores.
+__device__ __forceinline__ void cluster_leave() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ float4 peer_floats(uint32_t smem, uint32_t rank) {
     float4 v;
     asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
             }
         }
         __syncwarp();
-        cluster_sync();  // nobody leaves while its sums are being read
+        cluster_leave();  // nobody leaves while its sums are being read
     }
     tc_fence_before();
     __syncthreads();
