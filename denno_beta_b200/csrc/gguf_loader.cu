@@ -76,6 +76,7 @@ static uint64_t gguf_tensor_bytes(int type, const uint64_t* dims, int n_dims) {
     if (type == 0) return n * 4;   // F32
     if (type == 1) return n * 2;   // F16
     if (type == 30) return n * 2;  // BF16
+    if (type == T_MXFP4) return dims[0] % 32 ? 0 : n / 32 * 17;  // 4-bit microscaled: dnb_mx4_quantize_dev lays its blocks out for the products
     const int be = block_elems(type), ts = type_size(type);
     if (be == 0 || ts == 0 || dims[0] % (uint64_t)be) return 0;
     return n / be * ts;

@@ -194,7 +194,8 @@ int dnb_set_router_tc(dnb_ctx* ctx, int on);
  *   dnb_mx4_quantize_dev: rows of F32, F16 or BF16, ldx elements apart (aligned as their type), to such a matrix.  The scale's
  *       exponent is floor(log2(largest magnitude of the 32)) - 2, at least -127; elements are rounded to nearest, ties to
  *       even, and to 6 beyond it.  32 elements with an infinity or a NaN among them get scale 255 and codes of zero.
- *       Type MXFP4: rows of a GGUF file's 17-byte blocks, laid out anew (weights: once, as they are loaded); ldx a multiple of 32.
+ *       Type MXFP4: rows of a GGUF file's 17-byte blocks (dnb_gguf_tensor_data), laid out anew (weights: once, as they are loaded);
+ *       ldx a multiple of 32.
  *   dnb_mx4_dequantize_dev: back to F32 or BF16 (exact, but for overflow) or F16 (rounded), rows ldo elements apart.
  *   dnb_mx4_gemm_dev: out[t][r] = sum_i X[t][i] W[r][i] for nt rows X and n rows W, out F32, F16 or BF16.  Products are exact, sums 32 bits.
  *   dnb_mx4_gated_dev: out[t][r] = act(g) * u with g = sum_i X[t][i] G[r][i], u = sum_i X[t][i] U[r][i] (cf. dnb_moe_experts); out as

@@ -324,3 +324,100 @@ def test_no_rows(cu, ctx):
     assert ctx.launch_count() == before
     torch.cuda.synchronize()
     assert bool((out == 5).all())
+
+
+def test_two_contexts_at_once(cu):
+    """Two contexts, each on a stream of its own, with products of both sizes in flight together: each gives what it gives alone."""
+    gen = torch.Generator().manual_seed(6)
+    work = []
+    for i, shapes in enumerate((((2000, 512, 2100), (7, 2048, 3000)), ((1500, 768, 1800), (100, 1024, 2000)))):
+        c, stream, jobs = cu.CudaCtx(0), torch.cuda.Stream(), []
+        c.set_stream(stream.cuda_stream)
+        for nt, k, n in shapes:
+            x, w = dh.pack(*dh.random_codes(gen, nt, k)), dh.pack(*dh.random_codes(gen, n, k))
+            jobs.append((nt, k, n, x, w, torch.empty(nt, n, device="cuda")))
+        work.append((c, stream, jobs))
+
+    def enqueue(c, jobs):
+        for nt, k, n, x, w, out in jobs:
+            assert c.mx4_gemm_dev(x[0].data_ptr(), x[1].data_ptr(), w[0].data_ptr(), w[1].data_ptr(), nt, k, n, cu.F32, out.data_ptr())
+
+    torch.cuda.synchronize()
+    alone = []
+    for c, _, jobs in work:
+        enqueue(c, jobs)
+        torch.cuda.synchronize()
+        alone.append([j[-1].clone() for j in jobs])
+        for j in jobs:
+            j[-1].zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, _, jobs in work:
+            enqueue(c, jobs)
+    torch.cuda.synchronize()
+    for (c, _, jobs), want in zip(work, alone):
+        assert c.device_status() == 0
+        assert all(torch.equal(j[-1], v) for j, v in zip(jobs, want))
+        c.close()
+
+
+def test_waits_for_what_is_before_it_on_its_stream(cu, ctx):
+    """An operand that a long kernel writes just before, on the same stream that is not torch's own, is the one that is used."""
+    gen = torch.Generator().manual_seed(2)
+    nt, k, n = 200, 256, 300
+    x, w = dh.pack(*dh.random_codes(gen, nt, k)), dh.pack(*dh.random_codes(gen, n, k))
+    want, out = torch.empty(nt, n, device="cuda"), torch.empty(nt, n, device="cuda")
+    args = lambda o, c, s: (c.data_ptr(), s.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), nt, k, n, cu.F32, o.data_ptr())  # noqa: E731
+    assert ctx.mx4_gemm_dev(*args(want, *x))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    late = torch.zeros_like(x[0]), torch.zeros_like(x[1])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        ctx.stall(3.0)
+        late[0].copy_(x[0])
+        late[1].copy_(x[1])
+        assert ctx.mx4_gemm_dev(*args(out, *late))
+        late[0].zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    ctx.set_stream(1)
+
+
+def test_first_calls_inside_a_capture():
+    """In a process that has not launched any of them: kernels are loaded and devices asked while the stream is being captured."""
+    import subprocess
+    import sys
+
+    text = """
+import sys
+sys.path[:0] = %r
+import torch
+from denno_beta_b200 import cuda as cu
+c, stream = cu.CudaCtx(0), torch.cuda.Stream()
+c.set_stream(stream.cuda_stream)
+x, w = torch.randn(300, 256, device="cuda"), torch.randn(400, 256, device="cuda")
+m = lambda rows: [torch.empty(n, dtype=torch.uint8, device="cuda") for n in cu.mx4_bytes(rows, 256)]
+xm, wm = m(300), m(400)
+many, few = torch.empty(300, 400, device="cuda"), torch.empty(3, 400, device="cuda")
+p = lambda v: [t.data_ptr() for t in v]
+def calls():
+    assert c.mx4_quantize_dev(cu.F32, x.data_ptr(), 300, 256, *p(xm)) and c.mx4_quantize_dev(cu.F32, w.data_ptr(), 400, 256, *p(wm))
+    assert c.mx4_gemm_dev(*p(xm), *p(wm), 300, 256, 400, cu.F32, many.data_ptr())
+    assert c.mx4_gemm_dev(*p(xm), *p(wm), 3, 256, 400, cu.F32, few.data_ptr())
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=stream):
+    calls()
+g.replay()
+torch.cuda.synchronize()
+a, b = many.clone(), few.clone()
+many.zero_(), few.zero_()
+calls()
+torch.cuda.synchronize()
+assert torch.equal(a, many) and torch.equal(b, few) and bool(a.any()) and torch.equal(a[:3], b)
+print("same")
+""" % (sys.path,)
+    got = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "same" in got.stdout, got.stderr[-2000:]
