@@ -35,6 +35,7 @@ struct Params {
     int M, N, K;
     int passes;                     // 2: the sum goes on over a[1], b[1]
     int splits;
+    int bn;                         // rows of B that are loaded and multiplied: N rounded up to 16
     int idesc_type;                 // 16 bit: 0 fp16, 1 bf16
     int out_type, act;
     void* out;
@@ -178,7 +179,7 @@ __device__ __forceinline__ void tile_out(const Params& p, int tile, uint32_t tac
     const int m = tile * TM + quad * 32 + lane;
     const uint32_t ta = tacc + ((uint32_t)(quad * 32) << 16);
 #pragma unroll 1
-    for (int g = half; g < C::BN / 16; g += 2) {
+    for (int g = half; 16 * g < p.N; g += 2) {
         uint32_t v0[16], v1[16];
         tmem_ld16(ta + 16 * g, v0);
         if constexpr (C::NA == 2) tmem_ld16(ta + C::BN + 16 * g, v1);
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
                     uint8_t* s = smem + st * C::STAGE;
                     const int pass = c >= kch, kc = pass ? c - kch : c;
                     const int kbs = C::FP4 ? min(2, nkb - 2 * kc) : 0;
-                    mb_expect_tx(&full[st], (uint32_t)(C::NA * C::A_BYTES + C::B_BYTES + (C::NA + 1) * kbs * 512));
+                    mb_expect_tx(&full[st], (uint32_t)(C::NA * C::A_BYTES + p.bn * 128 + (C::NA + 1) * kbs * 512));
 #pragma unroll
                     for (int a = 0; a < C::NA; ++a) {
                         const CUtensorMap* map = &p.a[C::NA == 2 ? a : pass];
@@ -361,9 +362,9 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
         const uint32_t sf_tmem = tmem + C::BUFS * C::ACC;
         uint32_t idesc;
         if constexpr (C::FP4)  // e2m1 operands, 2^x scales
-            idesc = (1u << 7) | (1u << 10) | ((uint32_t)(C::BN >> 3) << 17) | (1u << 23) | (1u << 27);
+            idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | (1u << 23) | (1u << 27);
         else
-            idesc = (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) | ((uint32_t)(C::BN >> 3) << 17) |
+            idesc = (1u << 4) | ((uint32_t)p.idesc_type << 7) | ((uint32_t)p.idesc_type << 10) | ((uint32_t)C::AMN << 15) | ((uint32_t)(p.bn >> 3) << 17) |
                     ((uint32_t)(TM >> 4) << 24);
         int it = 0, nt = 0;
         for (int t = first; t < tiles && ok; t += step, ++nt) {
@@ -538,10 +539,11 @@ int best_splits(dnb_ctx* c, int tiles, int chunks) {
 template <class C>
 int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* b, int nb, int type, const char* name) {
     int rc;
+    p.bn = (p.N + 15) / 16 * 16;
     for (int i = 0; i < na; ++i)
         if ((rc = operand_map<C::FP4>(&p.a[i], a[i], C::AMN ? 64 : TM, type))) return rc;
     for (int i = 0; i < nb; ++i)
-        if ((rc = operand_map<C::FP4>(&p.b[i], b[i], C::BN, type))) return rc;
+        if ((rc = operand_map<C::FP4>(&p.b[i], b[i], p.bn, type))) return rc;
     p.idesc_type = type == T_BF16;
     p.status = c->status;
     const int tiles = (p.M + TM - 1) / TM, chunks = (p.K + C::BK - 1) / C::BK * p.passes;
