@@ -90,7 +90,6 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, u
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int MORE>
 __device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(MORE) : "memory"); }
-__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Says that tensor memory has been read (tcgen05's wait and fence stand before it).  Released at the cluster's scope it would wait 1,300 cycles for
 // the stores of the last tile, which nobody has to see.
 __device__ __forceinline__ void remote_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
@@ -499,12 +498,15 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
                 }
             }
         }
-        if (lane == 0) store_done();
+        if (lane == 0) store_read<0>();  // the boxes have been read
     }
     __syncwarp();
     __syncwarp();
     tc_fence_before();
-    cluster_sync();  // nobody's shared or tensor memory goes while the other may still use it
+    // Nobody's shared or tensor memory goes while another may still use it.  After a split tile only reads are left: the last arrivals at another
+    // CTA's barriers came before the shares were waited for.
+    if (shares) cluster_leave();
+    else cluster_sync();
     if (warp == 1) {
         tc_fence_after();
         pair_free(tmem);
