@@ -104,7 +104,7 @@ def test_both_directions(cu, ctx, act, name, nt, k, n):
         assert bool((b.out[:, n:] == 7).all()) and bool((b.dx[:, k:] == 7).all())
 
 
-@pytest.mark.parametrize("nt,k,n", [(77, 2056, 5640), (3000, 72, 2056), (8, 4096, 4096), (2000, 2048, 136)])
+@pytest.mark.parametrize("nt,k,n", [(77, 2056, 5640), (3000, 72, 2056), (8, 4096, 4096), (2000, 2048, 136), (2900, 2048, 264), (2600, 2304, 1408), (4700, 640, 1032)])
 def test_many_tiles(cu, ctx, nt, k, n):
     """Several tiles for every SM, with next to nothing between them: sums of the kernel's own 16-bit operands, every time the same bits."""
     b = Block(cu, "silu", "bf16", nt, k, n)
