@@ -5,13 +5,20 @@
 // Gated: the B tile is 128 rows of gate in one CTA and the same 128 of up in the other, so that a thread that reads a row of D has g and u
 // of the same features: 256 x 128 results from one MMA.
 // Operands as in dense_tc.cuh: 4 bits with scales in tensor memory, or 16 bits with rows along K or along m / n.
+//
 // Tiles go to the pairs in turn.  What is left over when every pair has had as many, or all of them where there are few, one tile a cluster of
 // two to four pairs: these divide K, and each CTA adds up some of the columns, the pairs' shares in ascending order, through distributed shared memory.
 //
-// A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight
-// warps read the accumulators: a thread a row, 32 columns at a time, through 4 KB of shared memory a warp and out by TMA stores (or, where
-// rows do not start or end at multiples of 16 bytes, in whole rows by plain stores).  16 bits: two accumulators; 4 bits, where the scales take the
-// room: one, drained to registers at once so that the next tile's MMAs need not wait for the stores.
+// A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight warps
+// read the accumulators: a thread a row, its 128 columns at once, then 64 (16 bits) or 32 at a time through 4 KB of shared memory a warp and out by TMA
+// stores (rows that do not start or end at multiples of 16 bytes: by plain stores, a row a warp).  16 bits: two accumulators; 4 bits, where the scales
+// take the room: one, in registers before the next tile's MMAs need it.
+//
+// What bounds it.  A chunk (64 of K in 16 bits, 256 in 4) takes 615 and 650 cycles where its MMAs alone take 512: 54 bytes a clock come into an SM,
+// of 64 that its port takes.  Two tiles that share a B (384 rows a stage, 47 bytes a clock) were 1.5 to 5 % faster on long runs, no faster on short ones,
+// and are not kept.  Long runs are bound by the power limit: bf16 4096 tokens, 4096 -> 10240, 1.57 PFLOP/s for some milliseconds (0.93 of the measured
+// peak), 1.36 at 1.2 to 1.35 GHz; 4 bits, 8192 tokens, 4096 -> 8192, 104 us (5.3 PFLOP/s), 129 at 1.6 GHz.  Short ones: about 5 us of launch, set-up and
+// first copies, and a first tile's epilogue of 2,500 cycles (1,100 once its code is in the instruction cache).
 #pragma once
 #include <type_traits>
 
@@ -559,7 +566,8 @@ int pair_clusters(dnb_ctx* c, int parts) {
     return n;
 }
 // Pairs a cluster and how many tiles are not split.  A tile costs its chunks of K and about four more; a split one a part of the chunks and about
-// ten (shares written, the cluster waited for, sums read).
+// ten (shares written, the cluster waited for, sums read).  us a call without / with: dx of 256 tokens, 2048 -> 5632 (8 tiles of 176 chunks) 65 / 31, of
+// 1024 tokens 66 / 43; 4-bit 512 tokens, 12288 -> 4096 (32 tiles of 48) 23.8 / 18; gated 512 tokens, 2560 -> 9728 in fp16 (152 tiles of 40) 48.4 / 46.
 template <class C>
 void choose_parts(dnb_ctx* c, int tiles, int chunks, int& parts, int& whole, int& clusters) {
     float least = 0.f;
