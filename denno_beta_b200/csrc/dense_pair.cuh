@@ -78,6 +78,7 @@ struct Cfg {
     static constexpr int COLS = 512;
     static constexpr int NOUT = GATED ? 128 : 256;             // columns of the output a tile
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + STAGING + 1024 + 256;
+    static_assert(SMEM > kBesideNone && SMEM <= 232448, "alone on its SM");
 };
 
 // ---- PTX of pairs ---------------------------------------------------------------------------------------------------------------
@@ -164,26 +165,28 @@ __device__ __forceinline__ void halves(const float (&v)[32], uint32_t (&h)[16]) 
 #pragma unroll
     for (int i = 0; i < 16; ++i) h[i] = two<OUT>(v[2 * i], v[2 * i + 1]);
 }
-// Before chunk_put: another of the warp's boxes, which has been read by now.
+// A warp's boxes take turns: one is written when all groups of stores but the last have been read.  So every chunk is a group, stored by TMA or not.
+struct Boxes {
+    uint8_t* base;
+    uint32_t at;  // 0 or 4096
+};
 template <class C>
-__device__ __forceinline__ void chunk_begin(int lane, uint8_t*& buf) {
-    if constexpr (C::BOXES == 2) buf = reinterpret_cast<uint8_t*>(reinterpret_cast<uintptr_t>(buf) ^ 4096);
+__device__ __forceinline__ uint8_t* chunk_begin(int lane, Boxes& b) {
+    if constexpr (C::BOXES == 2) b.at ^= 4096;
     if (lane == 0) store_read<C::BOXES - 1>();
     __syncwarp();
+    return b.base + b.at;
 }
 // From (row0, col0) of a [M][N] matrix.
 template <int OUT>
-__device__ __forceinline__ void chunk_end(const CUtensorMap* map, bool tma, void* out, size_t ldo, int M, int N, int row0, int col0, uint8_t* buf, int lane) {
-    if (tma) {
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-            if (row0 < M && col0 < N) store_2d(map, col0, row0, s32(buf));
-            store_commit();  // a group for each box, whether or not it has anything to store: they are counted
-        }
-        return;
-    }
+__device__ __forceinline__ void chunk_end(const CUtensorMap* map, bool tma, void* out, size_t ldo, int M, int N, int row0, int col0, const uint8_t* buf, int lane) {
+    if (tma) fence_async_smem();
     __syncwarp();
+    if (lane == 0) {
+        if (tma && row0 < M && col0 < N) store_2d(map, col0, row0, s32(buf));
+        store_commit();
+    }
+    if (tma) return;
     const int rows = min(32, M - row0);
     constexpr int SIZE = OUT == T_F32 ? 4 : 2;
     using W = typename std::conditional<OUT == T_F32, float, uint16_t>::type;
@@ -217,14 +220,14 @@ __device__ __forceinline__ void block_out(const Params& p, int row, int col, con
 
 // What a thread does with 32 columns (gated: of g and of u) from `col`: chunk c of its row.
 template <class C, int OUT>
-__device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which, int c, int row0, int col, float (&g)[32], float (&u)[32], uint8_t*& buf, int lane,
+__device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which, int c, int row0, int col, float (&g)[32], float (&u)[32], Boxes& boxes, int lane,
                                          uint32_t (&first)[16]) {
     if constexpr (C::GATED) {
         if (p.keep) {
-            chunk_begin<C>(lane, buf);
+            uint8_t* buf = chunk_begin<C>(lane, boxes);
             chunk_put(buf, lane, g);
             chunk_end<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
-            chunk_begin<C>(lane, buf);
+            buf = chunk_begin<C>(lane, boxes);
             chunk_put(buf, lane, u);
             chunk_end<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
         }
@@ -234,7 +237,7 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
     if constexpr (OUT == T_MXFP4) {
         block_out(p, row0 + lane, col, g);
     } else if constexpr (OUT == T_F32) {
-        chunk_begin<C>(lane, buf);
+        uint8_t* buf = chunk_begin<C>(lane, boxes);
         chunk_put(buf, lane, g);
         chunk_end<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col, buf, lane);
     } else {
@@ -242,7 +245,7 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
         if ((c & 1) == 0) return halves<OUT>(g, first);
         uint32_t h[16];
         halves<OUT>(g, h);
-        chunk_begin<C>(lane, buf);
+        uint8_t* buf = chunk_begin<C>(lane, boxes);
         chunk_put(buf, lane, 0, first);
         chunk_put(buf, lane, 1, h);
         chunk_end<OUT>(&p.out[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row0, col - 32, buf, lane);
@@ -251,13 +254,13 @@ __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which
 
 // This thread's part of a tile, 128 columns (gated: 64 of g and of u), in registers: every element by a constant index, so the chunks are unrolled.
 template <class C, int OUT>
-__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, uint8_t*& buf, int lane, float (&v)[4][32]) {
+__device__ __forceinline__ void results(const Params& p, int which, int row0, int n0, int half, Boxes& boxes, int lane, float (&v)[4][32]) {
     constexpr int CHUNKS = C::GATED ? 2 : 4;
     const ActForm act = act_form(p.act);
     uint32_t first[16];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
-        chunk_of<C, OUT>(p, act, which, c, row0, n0 + 32 * (half * CHUNKS + c), v[c], v[C::GATED ? 2 + c : c], buf, lane, first);
+        chunk_of<C, OUT>(p, act, which, c, row0, n0 + 32 * (half * CHUNKS + c), v[c], v[C::GATED ? 2 + c : c], boxes, lane, first);
 }
 
 // A split tile.  This CTA's sums in the ring's memory, four columns of all rows after another: what a warp reads of another CTA's is 512 bytes in a
@@ -265,7 +268,7 @@ __device__ __forceinline__ void results(const Params& p, int which, int row0, in
 __device__ __forceinline__ uint32_t share_at(int row, int unit) { return (uint32_t)(unit * 128 + row) * 16; }
 // 64 columns of the output (a warp 32 rows of them), summed over the cluster's pairs.
 template <class C, int OUT>
-__device__ __forceinline__ void joined(const Params& p, int which, int quad, int row0, int n0, int unit, uint32_t share, uint32_t rank, uint8_t*& buf, int lane) {
+__device__ __forceinline__ void joined(const Params& p, int which, int quad, int row0, int n0, int unit, uint32_t share, uint32_t rank, Boxes& boxes, int lane) {
     const ActForm act = act_form(p.act);
     uint32_t first[16];
 #pragma unroll 1
@@ -289,7 +292,7 @@ __device__ __forceinline__ void joined(const Params& p, int which, int quad, int
                 }
             }
         }
-        chunk_of<C, OUT>(p, act, which, c, row0, n0 + col, v[0], v[C::GATED ? 1 : 0], buf, lane, first);
+        chunk_of<C, OUT>(p, act, which, c, row0, n0 + col, v[0], v[C::GATED ? 1 : 0], boxes, lane, first);
     }
 }
 
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
         // ---------------- results ----------------
         const int quad = warp & 3, half = (warp - 4) >> 2;
-        uint8_t* buf_s = staging + (warp - 4) * C::BOXES * 4096;
+        Boxes boxes = {staging + (warp - 4) * C::BOXES * 4096, 0};
         for (int nt = 0; nt < turns && ok; ++nt) {
             const int buf = nt % C::BUFS, use = nt / C::BUFS;
             // Where to is worked out before the wait: with one accumulator the next tile's MMAs wait for what is between it and the arrival.  All of a
@@ -484,10 +487,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
                 break;
             }
             switch (p.out_type) {
-                case T_F16: results<C, T_F16>(p, which, row0, n0, half, buf_s, lane, v); break;
-                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, buf_s, lane, v); break;
-                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, buf_s, lane, v); break;
-                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, buf_s, lane, v);
+                case T_F16: results<C, T_F16>(p, which, row0, n0, half, boxes, lane, v); break;
+                case T_BF16: results<C, T_BF16>(p, which, row0, n0, half, boxes, lane, v); break;
+                case T_F32: if constexpr (C::FP4) results<C, T_F32>(p, which, row0, n0, half, boxes, lane, v); break;
+                default: if constexpr (C::FP4 && C::GATED) results<C, T_MXFP4>(p, which, row0, n0, half, boxes, lane, v);
             }
         }
         __syncwarp();
@@ -498,10 +501,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
             const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
             if (unit < C::NOUT / 64) {
                 switch (p.out_type) {
-                    case T_F16: joined<C, T_F16>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane); break;
-                    case T_BF16: joined<C, T_BF16>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane); break;
-                    case T_F32: if constexpr (C::FP4) joined<C, T_F32>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane); break;
-                    default: if constexpr (C::FP4 && C::GATED) joined<C, T_MXFP4>(p, which, quad, row0, n0, unit, s32(smem), rank, buf_s, lane);
+                    case T_F16: joined<C, T_F16>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane); break;
+                    case T_BF16: joined<C, T_BF16>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane); break;
+                    case T_F32: if constexpr (C::FP4) joined<C, T_F32>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane); break;
+                    default: if constexpr (C::FP4 && C::GATED) joined<C, T_MXFP4>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane);
                 }
             }
         }

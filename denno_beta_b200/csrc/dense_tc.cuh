@@ -53,6 +53,9 @@ struct Params {
     int* status;
 };
 
+// Blocks that share an SM never ask for more tensor memory together than it has (one would wait for the other, and clusters for one another): those
+// of half of it or less take over a third of an SM's 228 KB of shared memory, the others too much to stand beside one of those.
+constexpr size_t kOneOfTwo = 233472 / 3, kBesideNone = 233472 - kOneOfTwo - 2048;
 constexpr int pow2_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
 
 template <bool FP4_, int NA_, int BN_, bool AMN_ = false>
@@ -73,6 +76,7 @@ struct Cfg {
     static constexpr int COLS = pow2_cols(BUFS * ACC + 2 * SF_COLS);
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 512;
     static_assert(STAGES >= 2 && PER_SM * COLS <= 512, "no room");
+    static_assert(SMEM > (PER_SM == 2 ? kOneOfTwo : kBesideNone) && SMEM <= (PER_SM == 2 ? 115712 : 232448), "shares an SM with one block, or with none");
     static_assert(!FP4 || !AMN, "4-bit operands lie along K");
 };
 
@@ -505,8 +509,8 @@ cudaLaunchConfig_t launch_config(dnb_ctx* c, cudaLaunchAttribute (&at)[2], unsig
     return cfg;
 }
 
-// How many clusters of `splits` blocks the device holds at once: blocks of a cluster share a GPC, whose SMs they may not fill (16 clusters of eight
-// where 148 SMs could hold 18).  Asked once a device.
+// How many clusters of `splits` blocks the device holds at once: blocks of a cluster share a GPC, whose SMs they may not fill (15 clusters of eight
+// blocks that each want an SM, where 148 SMs could hold 18).  Asked once a device.
 template <class C>
 int clusters_at_once(dnb_ctx* c, int splits) {
     static std::atomic<int> known[64][9];

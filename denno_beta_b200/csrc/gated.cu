@@ -64,8 +64,8 @@ static int check_shape(const char* what, int act, int type, int nt, int k, int n
         set_error("%s: bad argument (activation %d, tokens %d, k %d, n %d)", what, act, nt, k, n);
         return DNB_ERR_ARG;
     }
-    if ((type != T_F16 && type != T_BF16) || k % 8 || n % 8) {
-        set_error("%s: ggml type %d with k=%d, n=%d is not handled (F16 or BF16, multiples of 8)", what, type, k, n);
+    if ((type != T_F16 && type != T_BF16) || k % 8 || n % 8 || nt > 1 << 30 || k > 1 << 30 || n > 1 << 30) {
+        set_error("%s: ggml type %d with %d tokens, k=%d, n=%d is not handled (F16 or BF16, k and n multiples of 8, up to 2^30)", what, type, nt, k, n);
         return DNB_DECLINED;
     }
     return DNB_OK;

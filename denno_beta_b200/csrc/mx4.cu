@@ -285,6 +285,13 @@ static int check_matrix(const char* what, const void* codes, const void* scales,
     return DNB_OK;
 }
 
+// Sizes that tiles are counted for in 32 bits.
+static int check_sizes(const char* what, int nt, int k, int n) {
+    if (nt <= 1 << 30 && k <= 1 << 30 && n <= 1 << 30) return DNB_OK;
+    set_error("%s: %d x %d x %d is more than one launch takes", what, nt, k, n);
+    return DNB_DECLINED;
+}
+
 // One product (NA 1) or the gated one (2).  Up to 128 tokens: narrow tiles of tokens under the weights' rows (dense_tc.cuh); beyond, tiles of
 // 256 tokens (dense_pair.cuh).
 template <int NA>
@@ -413,7 +420,7 @@ int dnb_mx4_gemm_dev(dnb_ctx* c, const void* xc, const void* xs, const void* wc,
         set_error("mx4_gemm: results of ggml type %d are not handled", type);
         return DNB_DECLINED;
     }
-    if (nt == 0) return DNB_OK;
+    if ((rc = check_sizes("mx4_gemm", nt, k, n)) || nt == 0) return rc;
     DNB_CUDA(cudaSetDevice(c->device));
     return product<1>(c, xc, xs, &wc, &ws, nt, k, n, ACT_NONE, type, out_dev, nullptr, ldo, "mx4_gemm");
 }
@@ -434,7 +441,7 @@ int dnb_mx4_gated_dev(dnb_ctx* c, int act, const void* xc, const void* xs, const
         set_error("mx4_gated: results of ggml type %d, %d a row, are not handled", type, n);
         return DNB_DECLINED;
     }
-    if (nt == 0) return DNB_OK;
+    if ((rc = check_sizes("mx4_gated", nt, k, n)) || nt == 0) return rc;
     DNB_CUDA(cudaSetDevice(c->device));
     const void *wc[2] = {gc, uc}, *ws[2] = {gs, us};
     return product<2>(c, xc, xs, wc, ws, nt, k, n, act, type, out_dev, (uint8_t*)out_scales_dev, ldo, "mx4_gated");

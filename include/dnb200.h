@@ -93,8 +93,8 @@ uint64_t dnb_launch_count(dnb_ctx* ctx);
  *   24       expert-parallel decode: a peer's result rows did not arrive
  *   23       grid barrier of the fused one-token kernel
  *   25       the tensor-core router GEMM of a prefill chunk (stage or accumulator barrier)
- *   27-29    a dense product (microscaled 4-bit or 16-bit): stage, accumulator or drain barrier
  *   26       no wait: a grouped kernel (mma.sync or tcgen05) found its shared memory to start elsewhere than the context has it
+ *   27-29    a dense product (microscaled 4-bit or 16-bit): stage, accumulator or drain barrier
  * What the reference promises for a GPU call that did not complete -- "false: out
  * untouched, the caller recomputes" (cuda.rs:21024-21027, 8785-8788) -- holds here too:
  * every host-buffer entry point reads the word after its stream synchronisation and, when
@@ -200,8 +200,8 @@ int dnb_set_router_tc(dnb_ctx* ctx, int on);
  *   dnb_mx4_gemm_dev: out[t][r] = sum_i X[t][i] W[r][i] for nt rows X and n rows W, out F32, F16 or BF16.  Products are exact, sums 32 bits.
  *   dnb_mx4_gated_dev: out[t][r] = act(g) * u with g = sum_i X[t][i] G[r][i], u = sum_i X[t][i] U[r][i] (cf. dnb_moe_experts); out as
  *       before, or MXFP4 with n a multiple of 32: quantised as above into out (codes) and out_scales, the operand of the next product.
- * The same inputs give the same bits on every run; a row's bits may depend on how many rows the call has (the sum over k is
- * divided among thread blocks where there are few). */
+ * The same inputs give the same bits on every run on a device; a row's bits may depend on how many rows the call has and on
+ * the device (the sum over k is divided among thread blocks where there are few, in as many parts as it holds at once). */
 #define DNB_ACT_SILU 0  /* v / (1 + exp(-v)) */
 #define DNB_ACT_GELU 1  /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
 int dnb_mx4_bytes(int rows, int k, size_t* codes, size_t* scales);
@@ -225,7 +225,7 @@ int dnb_mx4_gated_dev(dnb_ctx* ctx, int act, const void* x_codes, const void* x_
  *       dx [nt][k] = dpre[0] gate + dpre[1] up, or NULL (x is not looked at without the weights' gradients, nor gate and up without dx),
  *       dgate, dup [n][k] = dpre[0]^T x, dpre[1]^T x, or both NULL.  With nt = 0 they are zeros.
  * 4-bit weights have no gradient of their own; dx for them: dnb_mx4_dequantize_dev to BF16 is exact.
- * A row's bits may depend on nt, as above. */
+ * A row's bits may depend on nt and on the device, as above. */
 int dnb_gated_dev(dnb_ctx* ctx, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev, int nt, int k,
                   int n, void* out_dev, size_t ldo, float* pre_dev);
 int dnb_gated_backward_dev(dnb_ctx* ctx, int act, int type, const void* x_dev, size_t ldx, const void* gate_dev, const void* up_dev,

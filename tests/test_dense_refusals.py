@@ -59,7 +59,7 @@ def test_dequantise(lib, ctx, want, change):
 
 @pytest.mark.parametrize("want,change", [
     (ERR, dict(ctx=None)), (ERR, dict(xc=None)), (ERR, dict(ws=None)), (ERR, dict(nt=-1)), (ERR, dict(n=0)), (ERR, dict(n=-3)), (ERR, dict(out=None)),
-    (ERR, dict(ldo=9)), (DECLINED, dict(k=80)), (DECLINED, dict(xs=ODD)), (DECLINED, dict(wc=ODD)), (DECLINED, dict(ty=MX)), (DECLINED, dict(ty=Q4_K)),
+    (ERR, dict(ldo=9)), (DECLINED, dict(k=80)), (DECLINED, dict(n=(1 << 30) + 1, ldo=1 << 31)), (DECLINED, dict(nt=(1 << 30) + 1)), (DECLINED, dict(xs=ODD)), (DECLINED, dict(wc=ODD)), (DECLINED, dict(ty=MX)), (DECLINED, dict(ty=Q4_K)),
     (DECLINED, dict(ty=F16, out=P + 1)),
 ])
 def test_product(lib, ctx, want, change):
@@ -80,7 +80,7 @@ def test_gated4(lib, ctx, want, change):
 
 @pytest.mark.parametrize("want,change", [
     (ERR, dict(ctx=None)), (ERR, dict(act=5)), (ERR, dict(nt=-1)), (ERR, dict(n=0)), (ERR, dict(x=None)), (ERR, dict(g=None)), (ERR, dict(out=None)),
-    (ERR, dict(ldx=8)), (ERR, dict(ldo=8)), (DECLINED, dict(ty=F32)), (DECLINED, dict(ty=MX)), (DECLINED, dict(k=20, ldx=24)), (DECLINED, dict(n=12)),
+    (ERR, dict(ldx=8)), (ERR, dict(ldo=8)), (DECLINED, dict(ty=F32)), (DECLINED, dict(ty=MX)), (DECLINED, dict(k=20, ldx=24)), (DECLINED, dict(n=12)), (DECLINED, dict(n=(1 << 30) + 8, ldo=1 << 31)),
     (DECLINED, dict(x=ODD)), (DECLINED, dict(ldx=20)), (DECLINED, dict(u=ODD)), (DECLINED, dict(pre=ODD)), (DECLINED, dict(out=P + 1)),
 ])
 def test_gated(lib, ctx, want, change):

@@ -126,6 +126,27 @@ def test_many_tiles(cu, ctx, nt, k, n):
         assert int(((got.double() - want).abs() > off + dh.floor_of(b.t)).sum()) == 0
 
 
+@pytest.mark.parametrize("nt,k,n", [(3000, 64, 1032), (20, 1024, 264), (700, 2048, 136)])
+def test_results_off_their_alignment(cu, ctx, nt, k, n):
+    """out and dx at odd addresses with rows of odd distances, beside pre in 32 bits: the bits of the aligned call."""
+    b = Block(cu, "gelu", "bf16", nt, k, n)
+    assert b.forward(ctx) and b.backward(ctx)
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (b.out, b.pre, b.dx, b.dg, b.du)]
+    for _ in range(3):
+        out, dx = (torch.full((nt * (w + 5) + 1,), 9.0, dtype=b.t, device="cuda") for w in (n, k))
+        dg, du = (torch.full((n * k + 1,), 9.0, dtype=b.t, device="cuda") for _ in range(2))
+        b.pre.fill_(0)
+        assert ctx.gated_dev(*b.ids, b.x.data_ptr(), b.g.data_ptr(), b.u.data_ptr(), nt, k, n, out.data_ptr() + 2, b.pre.data_ptr(), 0, n + 5)
+        assert ctx.gated_backward_dev(*b.ids, b.x.data_ptr(), b.g.data_ptr(), b.u.data_ptr(), b.pre.data_ptr(), b.dout.data_ptr(), nt, k, n, b.dpre.data_ptr(),
+                                      dx.data_ptr() + 2, dg.data_ptr() + 2, du.data_ptr() + 2, 0, 0, k + 5)
+        torch.cuda.synchronize()
+        for got, w, width in ((out[1:].reshape(nt, n + 5), want[0], n), (dx[1:].reshape(nt, k + 5), want[2], k)):
+            assert torch.equal(got[:, :width], w) and bool((got[:, width:] == 9).all())
+        assert torch.equal(b.pre, want[1]) and torch.equal(dg[1:].reshape(n, k), want[3]) and torch.equal(du[1:].reshape(n, k), want[4])
+        assert all(float(t[0]) == 9 for t in (out, dx, dg, du))
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gradients_against_differences(cu, ctx, act):
     """Along random directions: (f(p + h d) - f(p - h d)) / 2 h in 64 bits against the kernel's gradients."""
