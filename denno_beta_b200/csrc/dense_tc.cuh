@@ -10,9 +10,9 @@
 // accumulators (two a row quarter).  Few results: a cluster splits K and its CTAs' partial sums are added through distributed shared
 // memory in ascending rank order (no workspace, no atomics: the same bits on every run).
 //
-// What bounds it: the weights' bytes, and for the smallest the launch.  4-bit 65536 x 4096 (142 MB) 8 tokens 28 us (5.1 TB/s); gated bf16, 4 tokens,
-// 4096 -> 10240 (168 MB) 33 us (5.1 TB/s: 240 blocks on 148 SMs end 28 to 39 us after the start); 4-bit 4096 x 4096, one token, 5.4 us: 2.3 from the
-// start to the first operands, 1.5 of products, 1.5 to join the parts and leave.
+// What bounds it: the weights' bytes, and for the smallest the launch.  4-bit 65536 x 8192 (285 MB) 16 tokens 47.4 us (6.0 TB/s), 65536 x 4096 8 tokens 27.3
+// (5.2); gated bf16, 4 tokens, 4096 -> 10240 (168 MB) 31.2 (5.4; lower tiles that would share the weights evenly over the SMs change nothing); 4-bit
+// 4096 x 4096, one token, 5.3: 2.3 from the start to the first operands, 1.5 of products, 1.5 to join the parts and leave.
 //
 // Up to 128 rows, as beyond that the other kernel's tiles are faster.  us a call here / there at 64, 96, 128 tokens: 4-bit 4096 x 4096 6.8 / 11.6, 7.8 / 11.8,
 // 8.1 / 11.9; 8192 -> 16384 18.6 / 19.8, 18.4 / 20.2, 19.6 / 20.5; gated bf16 4096 -> 10240 39 / 45, 44 / 45, 47 / 46; backward 2048 -> 5632 35 / 44, 35 /
@@ -486,10 +486,13 @@ struct Operand {  // a matrix in memory
     const void* data;
     uint64_t rows, cols, pitch;  // pitch: bytes between rows
 };
+// Boxes of 128 bytes a row, of which L2 fetches 256: a row's next box comes from the same page of memory.  8 % where the weights' bytes count: 4-bit 65536 x
+// 4096, 8 tokens, 29.2 us with 128 and 27.4 with 256; gated bf16, 4 tokens, 4096 -> 10240 34.0 and 31.2; no difference elsewhere.
 template <bool FP4>
 int operand_map(CUtensorMap* m, const Operand& o, int box_rows, int type) {
-    if constexpr (FP4) return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.data, o.rows, o.cols / 2, o.pitch, box_rows);
-    return tiled_map(m, type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.data, o.rows, o.cols, o.pitch, box_rows);
+    const CUtensorMapDataType t = FP4 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return tiled_map(m, t, FP4 ? 1 : 2, o.data, o.rows, FP4 ? o.cols / 2 : o.cols, o.pitch, box_rows, 0, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 template <class C>

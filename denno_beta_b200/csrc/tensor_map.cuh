@@ -20,9 +20,11 @@ inline EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// [rows][cols] of `type`, rows `pitch` bytes apart, in boxes of box_cols (0: 128 bytes) x box_rows; zeros beyond the matrix.
+// [rows][cols] of `type`, rows `pitch` bytes apart, in boxes of box_cols (0: 128 bytes) x box_rows; zeros beyond the matrix.  promotion: what L2
+// fetches at least.
 inline int tiled_map(CUtensorMap* m, CUtensorMapDataType type, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch,
-                     uint32_t box_rows, uint32_t box_cols = 0, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+                     uint32_t box_rows, uint32_t box_cols = 0, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B,
+                     CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
     const EncodeTiledFn fn = encode_fn();
     if (!fn) {
         set_error("cuTensorMapEncodeTiled is not available from this driver");
@@ -33,7 +35,7 @@ inline int tiled_map(CUtensorMap* m, CUtensorMapDataType type, int elem_bytes, c
     const cuuint32_t box[2] = {box_cols ? box_cols : (cuuint32_t)(128 / elem_bytes), box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled failed (%d) for %llu x %llu box %u", (int)r, (unsigned long long)rows, (unsigned long long)cols, box_rows);
         return DNB_ERR_CUDA;
