@@ -50,7 +50,9 @@ struct Params {
     int both;                       // 2: twice the tiles, the second half with a[1] to the second output
     int tiles_m, per_output;        // rows of tiles; tiles of one output
     Divisor group, last_group;      // tiles of eight rows of tiles; rows of the last group
-    int parts, whole;               // pairs a cluster; tiles that are not split (the rest: one a cluster)
+    int parts, whole, tiles;        // pairs a cluster; tiles that are not split (the rest: one a cluster); all
+    int each, more;                 // whole tiles a pair, one more for the first `more` pairs
+    int chunks, share[5];           // of K; the parts' first chunks of a split tile
     int idesc_type, out_type, act;
     bool tma_out, keep;             // keep: g and u to pre
     void* outp[2];
@@ -336,6 +338,12 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
     }
     if (warp == 0 && lane < 4) prefetch_map(lane < 2 ? &p.a[lane & ((p.passes | p.both) >> 1)] : &p.b[lane & (C::GATED ? 1 : p.passes >> 1)]);
     if (warp == 1) pair_alloc(tmem_slot);
+    // Turn i of this pair: a tile of its own, or its share of the cluster's tile, which is the last.  Worked out while the barriers are under way; the
+    // quotients come with the launch.
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1, chunks = p.chunks;
+    const int own = p.each + (first < p.more), split = p.whole + (int)cluster_id();
+    const bool shares = split < p.tiles;
+    const int turns = own + shares, s0 = p.share[part], s1 = p.share[part + 1];
     tc_fence_before();
     __syncthreads();
     cluster_sync();
@@ -344,13 +352,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
     pdl_wait();
     pdl_launch_dependents();
 
-    const int kch = (p.K + C::BK - 1) / C::BK, chunks = kch * p.passes, tiles = p.per_output * p.both;
-    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    // Turn i of this pair: a tile of its own, or its share of the cluster's tile, which is the last.
-    const int cluster = first / p.parts, own = first < p.whole ? (p.whole - first + step - 1) / step : 0;
-    const bool shares = p.whole + cluster < tiles;
-    const int turns = own + shares, split = p.whole + cluster;
-    const int s0 = (int)((long long)chunks * part / p.parts), s1 = (int)((long long)chunks * (part + 1) / p.parts);
     bool ok = true;
     int m, n, which;
 
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
         if (warp == 0) {
             // ---------------- TMA ----------------
-            const int nkb = (p.K + 127) >> 7;
+            const int nkb = (p.K + 127) >> 7, kch = p.passes == 2 ? chunks >> 1 : chunks;
             int it = 0;
             for (int i = 0; i < turns && ok; ++i) {
                 pair_tile(p, i < own ? first + i * step : split, m, n, which);
@@ -396,8 +397,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
                     __syncwarp();
                 }
             }
-            if (!ok && rank == 0)  // copies in flight, of both CTAs, end before their shared memory is given up
-                for (int i = max(0, it - C::STAGES); i < it; ++i) mb_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
+            // The last stages' arrivals, from the leader, come before the barriers that they arrive at go; if a wait gave up: the copies in flight, of both CTAs.
+            for (int i = max(0, it - C::STAGES); i < it && (ok || rank == 0); ++i)
+                mb_wait(ok ? &empty[i % C::STAGES] : &full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, kWaitStage);
         } else if (warp == 1) {
             // ---------------- MMA issue: the leader's thread for both ----------------
             if (rank == 0) {
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
                 tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) remote_arrive(drained);
+                if (lane == 0 && nt + C::BUFS < turns) remote_arrive(drained);  // where a later tile waits for it
             }
             if (nt == own) {  // the ring is empty: every copy has landed and been read
 #pragma unroll 1
@@ -513,10 +515,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
     __syncwarp();
     __syncwarp();
     tc_fence_before();
-    // Nobody's shared or tensor memory goes while another may still use it.  After a split tile only reads are left: the last arrivals at another
-    // CTA's barriers came before the shares were waited for.
-    if (shares) cluster_leave();
-    else cluster_sync();
+    // Nobody's shared or tensor memory goes while another may still use it: reads are over, and every arrival at another CTA's barrier has been waited for.
+    cluster_leave();
     if (warp == 1) {
         tc_fence_after();
         pair_free(tmem);
@@ -607,16 +607,21 @@ int launch_pair(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* 
         return DNB_DECLINED;
     }
     p.per_output = p.tiles_m * tiles_n;
+    p.tiles = (int)tiles;
+    p.chunks = (p.K + C::BK - 1) / C::BK * p.passes;
     p.group = divisor(8 * tiles_n);
     p.last_group = divisor(p.tiles_m % 8 ? p.tiles_m % 8 : 8);
     static SmemGrant grant;
     DNB_CUDA(grant_smem(grant, c->device, pair_kernel<C>, C::SMEM));
     int clusters;
-    choose_parts<C>(c, (int)tiles, (p.K + C::BK - 1) / C::BK * p.passes, p.parts, p.whole, clusters);
-    const int used = p.parts == 1 ? (int)tiles : p.whole > 0 ? clusters : (int)tiles;
+    choose_parts<C>(c, p.tiles, p.chunks, p.parts, p.whole, clusters);
+    const int used = p.parts > 1 && p.whole > 0 ? clusters : p.tiles < clusters ? p.tiles : clusters, pairs = used * p.parts;
+    p.each = p.whole / pairs;
+    p.more = p.whole % pairs;
+    for (int i = 0; i <= p.parts; ++i) p.share[i] = (int)((int64_t)p.chunks * i / p.parts);
     ProfScope prof_(c, c->stream, name);
     cudaLaunchAttribute at[2];
-    const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2u * p.parts * (unsigned)(used < clusters ? used : clusters), p.parts);
+    const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2u * (unsigned)pairs, p.parts);
     DNB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<C>, p));
     c->launches++;
     return DNB_OK;

@@ -42,7 +42,7 @@ struct Params {
     const uint8_t* sb;              // and of B
     int M, N, K;
     int passes;                     // 2: the sum goes on over a[1], b[1]
-    int splits;
+    int splits, chunks, share[9];   // parts of K, in chunks, and where each begins
     int bn;                         // rows of B that are loaded and multiplied: N rounded up to 16
     int idesc_type;                 // 16 bit: 0 fp16, 1 bf16
     int out_type, act;
@@ -142,6 +142,11 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatil
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_id() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -313,6 +318,9 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
     }
     if (warp == 0 && lane < 4) prefetch_map(lane < 2 ? &p.a[lane & (C::NA == 2 ? 1 : p.passes - 1)] : &p.b[lane & (p.passes - 1)]);
     if (warp == 1) tmem_alloc<C::COLS>(tmem_slot);
+    const int rank = p.splits > 1 ? (int)cluster_rank() : 0, c0 = p.share[rank], c1 = p.share[rank + 1], kch = p.passes == 2 ? p.chunks >> 1 : p.chunks;
+    const int tiles = (p.M + TM - 1) / TM, first = p.splits > 1 ? (int)cluster_id() : blockIdx.x, step = p.splits > 1 ? tiles : gridDim.x;
+    const int nkb = (p.K + 127) >> 7;  // scale tiles along K
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -320,12 +328,6 @@ __global__ void __launch_bounds__(NTHREADS, C::PER_SM) dense_kernel(const __grid
     pdl_wait();
     pdl_launch_dependents();
 
-    const int kch = (p.K + C::BK - 1) / C::BK, chunks = kch * p.passes;
-    const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
-    const int c0 = (int)((long long)chunks * rank / p.splits), c1 = (int)((long long)chunks * (rank + 1) / p.splits);
-    const int tiles = (p.M + TM - 1) / TM;
-    const int first = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, step = p.splits > 1 ? tiles : gridDim.x;
-    const int nkb = (p.K + 127) >> 7;  // scale tiles along K
     bool ok = true;
 
     if (warp == 0) {
@@ -566,6 +568,8 @@ int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand*
     static SmemGrant grant;
     DNB_CUDA(grant_smem(grant, c->device, dense_kernel<C>, C::SMEM));
     p.splits = best_splits<C>(c, tiles, chunks);
+    p.chunks = chunks;
+    for (int i = 0; i <= p.splits; ++i) p.share[i] = (int)((int64_t)chunks * i / p.splits);
     const int slots = c->sm_count * C::PER_SM;
     const unsigned grid = p.splits > 1 ? (unsigned)tiles * p.splits : (unsigned)(tiles < slots ? tiles : slots);
     ProfScope prof_(c, c->stream, name);
