@@ -14,7 +14,7 @@ using dt::Params;
 
 // A thread takes 8 elements of the rows r, r + 32, r + 64 and r + 96 of a tile of scales, 16 threads (half a warp) its 128 columns: four independent
 // 16- or 32-byte loads in flight a thread, and the 16 bytes of scales that these rows have next to each other are one store.  A block of 32 is four
-// neighbouring lanes.  Bound by memory: 14018 x 4096, fp32 to 4 bits 40 us (6.5 TB/s), bf16 29 (5.0) and back 29 (a row a thread at a time, 64-bit
+// neighbouring lanes.  Bound by memory: 14018 x 4096, fp32 to 4 bits 40 us (6.5 TB/s), bf16 29 (5.0) and back 26 (5.6; a row a thread at a time, 64-bit
 // divisions and a branch at each load, which waited for it: 47 and 37).
 constexpr int THREADS = 256, UNITS = THREADS / 16;
 
@@ -259,8 +259,11 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     }
 }
 
-static unsigned grid_of(const dnb_ctx* c, size_t units) {
-    const size_t want = (units + UNITS - 1) / UNITS, most = (size_t)c->sm_count * 8;
+// Blocks an SM, more than fit at once (4 and 6), so that the SMs end together; us for 14018 x 4096 bf16 with 4, 8, 16, 48 an SM: to 4 bits 30.0, 28.9, 29.1,
+// 32.2, back 33.7, 28.8, 26.0, 26.9.
+constexpr int TO_FOUR_BITS = 8, BACK = 16;
+static unsigned grid_of(const dnb_ctx* c, size_t units, int an_sm) {
+    const size_t want = (units + UNITS - 1) / UNITS, most = (size_t)c->sm_count * an_sm;
     return (unsigned)(want < most ? want : most);
 }
 
@@ -365,7 +368,7 @@ int dnb_mx4_quantize_dev(dnb_ctx* c, int type, const void* x_dev, size_t ldx, in
     DNB_CUDA(cudaSetDevice(c->device));
     const int nkb = (k + 127) / 128;
     const size_t folded = folded_rows(rows);
-    const dim3 grid(grid_of(c, folded * nkb)), block(THREADS);
+    const dim3 grid(grid_of(c, folded * nkb, TO_FOUR_BITS)), block(THREADS);
     const bool whole = aligned16(x_dev) && ldx * es % 16 == 0;
     uint8_t *codes = (uint8_t*)codes_dev, *scales = (uint8_t*)scales_dev;
     ProfScope prof_(c, c->stream, "mx4_quantize");
@@ -395,7 +398,7 @@ int dnb_mx4_dequantize_dev(dnb_ctx* c, const void* codes_dev, const void* scales
     DNB_CUDA(cudaSetDevice(c->device));
     const int nkb = (k + 127) / 128;
     const size_t folded = folded_rows(rows);
-    const dim3 grid(grid_of(c, folded * nkb)), block(THREADS);
+    const dim3 grid(grid_of(c, folded * nkb, BACK)), block(THREADS);
     const bool whole = aligned16(out_dev) && ldo * es % 16 == 0;
     const uint8_t *codes = (const uint8_t*)codes_dev, *scales = (const uint8_t*)scales_dev;
     ProfScope prof_(c, c->stream, "mx4_dequantize");
