@@ -7,7 +7,7 @@
 // Operands as in dense_tc.cuh: 4 bits with scales in tensor memory, or 16 bits with rows along K or along m / n.
 //
 // Tiles go to the pairs in turn.  What is left over when every pair has had as many, or all of them where there are few, one tile a cluster of
-// two to four pairs: these divide K, and each CTA adds up some of the columns, the pairs' shares in ascending order, through distributed shared memory.
+// two to four pairs: these divide K, and each CTA adds up some pieces of it, the pairs' shares in ascending order, through distributed shared memory.
 //
 // A CTA: warp 0 brings its halves by TMA (every copy reports to the leader's barrier), warp 1 of the leader issues the MMAs of both, eight warps
 // read the accumulators: a thread a row, its 128 columns at once, then 64 (16 bits) or 32 at a time through 4 KB of shared memory a warp and out by TMA
@@ -45,6 +45,7 @@ struct Params {
     CUtensorMap a[2], b[2];         // operands
     CUtensorMap sa, sb[2];          // scale tiles, 512 bytes a row (4 bit)
     CUtensorMap out[2], pre[2];     // results
+    CUtensorMap narrow[2];          // 16-bit results of split tiles, in boxes of 32 columns
     int M, N, K;                    // N: columns of the output
     int passes;                     // 2: the sum goes on over a[1], b[1]
     int both;                       // 2: twice the tiles, the second half with a[1] to the second output
@@ -157,6 +158,11 @@ __device__ __forceinline__ void chunk_put(uint8_t* buf, int lane, const float (&
 #pragma unroll
     for (int c = 0; c < 8; ++c) *reinterpret_cast<float4*>(row + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
+__device__ __forceinline__ void chunk_put(uint8_t* buf, int lane, const uint32_t (&h)[16]) {  // a row of 64 bytes
+    uint8_t* row = buf + lane * 64;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(row + ((c ^ (lane >> 1 & 3)) << 4)) = make_uint4(h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+}
 __device__ __forceinline__ void chunk_put(uint8_t* buf, int lane, int part, const uint32_t (&h)[16]) {  // 16 bits: one of two halves of a row
     uint8_t* row = buf + lane * 128;
 #pragma unroll
@@ -179,8 +185,8 @@ __device__ __forceinline__ uint8_t* chunk_begin(int lane, Boxes& b) {
     __syncwarp();
     return b.base + b.at;
 }
-// From (row0, col0) of a [M][N] matrix.
-template <int OUT>
+// From (row0, col0) of a [M][N] matrix, rows of BYTES.
+template <int OUT, int BYTES = 128>
 __device__ __forceinline__ void chunk_end(const CUtensorMap* map, bool tma, void* out, size_t ldo, int M, int N, int row0, int col0, const uint8_t* buf, int lane) {
     if (tma) fence_async_smem();
     __syncwarp();
@@ -193,12 +199,12 @@ __device__ __forceinline__ void chunk_end(const CUtensorMap* map, bool tma, void
     constexpr int SIZE = OUT == T_F32 ? 4 : 2;
     using W = typename std::conditional<OUT == T_F32, float, uint16_t>::type;
 #pragma unroll
-    for (int i = 0; i < 4 / SIZE; ++i) {
+    for (int i = 0; i < BYTES / SIZE / 32; ++i) {
         const int c = 32 * i + lane;
         if (col0 + c >= N) break;
         W* to = reinterpret_cast<W*>(out) + (size_t)row0 * ldo + col0 + c;
 #pragma unroll 8
-        for (int r = 0; r < rows; ++r) to[r * ldo] = *reinterpret_cast<const W*>(buf + r * 128 + (((c * SIZE >> 4) ^ (r & 7)) << 4) + (c * SIZE & 15));
+        for (int r = 0; r < rows; ++r) to[r * ldo] = *reinterpret_cast<const W*>(buf + r * BYTES + (((c * SIZE >> 4) ^ (BYTES == 128 ? r & 7 : r >> 1 & 3)) << 4) + (c * SIZE & 15));
     }
     __syncwarp();
 }
@@ -220,22 +226,25 @@ __device__ __forceinline__ void block_out(const Params& p, int row, int col, con
     p.out_scales[scale_at(row, col >> 5, (p.N + 127) >> 7)] = (uint8_t)(col < p.N ? e : 0u);
 }
 
+// 32 columns of g and u: kept, and g becomes the output.
+template <class C>
+__device__ __forceinline__ void gated_chunk(const Params& p, ActForm act, int row0, int col, float (&g)[32], float (&u)[32], Boxes& boxes, int lane) {
+    if (p.keep) {
+        uint8_t* buf = chunk_begin<C>(lane, boxes);
+        chunk_put(buf, lane, g);
+        chunk_end<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
+        buf = chunk_begin<C>(lane, boxes);
+        chunk_put(buf, lane, u);
+        chunk_end<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) g[j] = act_of(act, g[j]) * u[j];
+}
 // What a thread does with 32 columns (gated: of g and of u) from `col`: chunk c of its row.
 template <class C, int OUT>
 __device__ __forceinline__ void chunk_of(const Params& p, ActForm act, int which, int c, int row0, int col, float (&g)[32], float (&u)[32], Boxes& boxes, int lane,
                                          uint32_t (&first)[16]) {
-    if constexpr (C::GATED) {
-        if (p.keep) {
-            uint8_t* buf = chunk_begin<C>(lane, boxes);
-            chunk_put(buf, lane, g);
-            chunk_end<T_F32>(&p.pre[0], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
-            buf = chunk_begin<C>(lane, boxes);
-            chunk_put(buf, lane, u);
-            chunk_end<T_F32>(&p.pre[1], true, nullptr, 0, p.M, p.N, row0, col, buf, lane);
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) g[j] = act_of(act, g[j]) * u[j];
-    }
+    if constexpr (C::GATED) gated_chunk<C>(p, act, row0, col, g, u, boxes, lane);
     if constexpr (OUT == T_MXFP4) {
         block_out(p, row0 + lane, col, g);
     } else if constexpr (OUT == T_F32) {
@@ -268,33 +277,46 @@ __device__ __forceinline__ void results(const Params& p, int which, int row0, in
 // A split tile.  This CTA's sums in the ring's memory, four columns of all rows after another: what a warp reads of another CTA's is 512 bytes in a
 // row (16 bytes a row apart took twice as long).
 __device__ __forceinline__ uint32_t share_at(int row, int unit) { return (uint32_t)(unit * 128 + row) * 16; }
-// 64 columns of the output (a warp 32 rows of them), summed over the cluster's pairs.
+// The output of this CTA's 128 rows in pieces of 32 rows x 32 columns, a row a lane, summed over the cluster's pairs.  Neighbouring pieces go to
+// different pairs: all SMs read, with as many warps as there are pieces for; each asks another CTA first (all the same one: 7 % of a call) and
+// adds in ascending order.
 template <class C, int OUT>
-__device__ __forceinline__ void joined(const Params& p, int which, int quad, int row0, int n0, int unit, uint32_t share, uint32_t rank, Boxes& boxes, int lane) {
+__device__ __forceinline__ void joined(const Params& p, int which, int part, int warp, int row0, int n0, uint32_t share, uint32_t rank, Boxes& boxes, int lane) {
     const ActForm act = act_form(p.act);
-    uint32_t first[16];
 #pragma unroll 1
-    for (int c = 0; c < 2; ++c) {
-        const int col = 64 * unit + 32 * c;
+    for (int piece = part + p.parts * warp; piece < C::NOUT / 8; piece += p.parts * EPI_WARPS) {
+        const int r32 = (piece & 3) * 32, left = 32 * (piece >> 2), row = row0 + r32, col = n0 + left;
         float v[C::GATED ? 2 : 1][32];
 #pragma unroll
         for (int a = 0; a < (C::GATED ? 2 : 1); ++a) {
+            float t[4][32];
 #pragma unroll 1
-            for (int r = 0; r < p.parts; ++r) {
-                float4 t[8];  // all asked for before the first is added
+            for (int j = 0, r = part; j < p.parts; ++j, r = r + 1 < p.parts ? r + 1 : 0)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = peer_floats(share + share_at(quad * 32 + lane, (a * 128 + col) / 4 + i), 2 * r + rank);
+                for (int s = 0; s < 4; ++s)
+                    if (r == s) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float* s = &v[a][4 * i];
-                    s[0] = r ? s[0] + t[i].x : t[i].x;
-                    s[1] = r ? s[1] + t[i].y : t[i].y;
-                    s[2] = r ? s[2] + t[i].z : t[i].z;
-                    s[3] = r ? s[3] + t[i].w : t[i].w;
-                }
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(&t[s][4 * i]) = peer_floats(share + share_at(r32 + lane, (a * 128 + left) / 4 + i), 2 * s + rank);
+                    }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                v[a][i] = t[0][i] + t[1][i];
+                if (p.parts > 2) v[a][i] += t[2][i];
+                if (p.parts > 3) v[a][i] += t[3][i];
             }
         }
-        chunk_of<C, OUT>(p, act, which, c, row0, n0 + col, v[0], v[C::GATED ? 1 : 0], boxes, lane, first);
+        if constexpr (OUT == T_F16 || OUT == T_BF16) {
+            if constexpr (C::GATED) gated_chunk<C>(p, act, row, col, v[0], v[1], boxes, lane);
+            uint32_t h[16];
+            halves<OUT>(v[0], h);
+            uint8_t* buf = chunk_begin<C>(lane, boxes);
+            chunk_put(buf, lane, h);
+            chunk_end<OUT, 64>(&p.narrow[which], p.tma_out, p.outp[which], p.ldo, p.M, p.N, row, col, buf, lane);
+        } else {
+            uint32_t unused[16];
+            chunk_of<C, OUT>(p, act, which, 0, row, col, v[0], v[C::GATED ? 1 : 0], boxes, lane, unused);
+        }
     }
 }
 
@@ -498,16 +520,14 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
         __syncwarp();
         if (shares) {  // the whole cluster: those of the other warps wait below
             cluster_sync();
-            const int unit = (int)part + half * p.parts;
             pair_tile(p, split, m, n, which);
-            const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * C::NOUT;
-            if (unit < C::NOUT / 64) {
-                switch (p.out_type) {
-                    case T_F16: joined<C, T_F16>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane); break;
-                    case T_BF16: joined<C, T_BF16>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane); break;
-                    case T_F32: if constexpr (C::FP4) joined<C, T_F32>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane); break;
-                    default: if constexpr (C::FP4 && C::GATED) joined<C, T_MXFP4>(p, which, quad, row0, n0, unit, s32(smem), rank, boxes, lane);
-                }
+            const int row0 = m * 256 + (int)rank * 128, n0 = n * C::NOUT;
+            const uint32_t sums = s32(smem);
+            switch (p.out_type) {
+                case T_F16: joined<C, T_F16>(p, which, part, warp - 4, row0, n0, sums, rank, boxes, lane); break;
+                case T_BF16: joined<C, T_BF16>(p, which, part, warp - 4, row0, n0, sums, rank, boxes, lane); break;
+                case T_F32: if constexpr (C::FP4) joined<C, T_F32>(p, which, part, warp - 4, row0, n0, sums, rank, boxes, lane); break;
+                default: if constexpr (C::FP4 && C::GATED) joined<C, T_MXFP4>(p, which, part, warp - 4, row0, n0, sums, rank, boxes, lane);
             }
         }
         if (lane == 0) store_read<0>();  // the boxes have been read
@@ -528,11 +548,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
 inline int scale_map(CUtensorMap* m, const void* scales, uint64_t rows, uint64_t k) {
     return tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, scales, (rows + 127) / 128 * ((k + 127) / 128), 128, 512, 2, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-// Results [rows][cols] of `type`, in the epilogue's boxes.
-inline int result_map(CUtensorMap* m, int type, const void* out, uint64_t rows, uint64_t cols, uint64_t ld) {
+// Results [rows][cols] of `type`, in the epilogue's boxes, rows of 128 bytes or (16-bit ones) 64.
+inline int result_map(CUtensorMap* m, int type, const void* out, uint64_t rows, uint64_t cols, uint64_t ld, int bytes = 128) {
     const bool f32 = type == T_F32;
     return tiled_map(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, f32 ? 4 : 2, out, rows,
-                     cols, ld * (f32 ? 4 : 2), 32);
+                     cols, ld * (f32 ? 4 : 2), 32, bytes / (f32 ? 4 : 2), bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <class C>
@@ -618,6 +638,8 @@ int launch_pair(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* 
     const int used = p.parts > 1 && p.whole > 0 ? clusters : p.tiles < clusters ? p.tiles : clusters, pairs = used * p.parts;
     p.each = p.whole / pairs;
     p.more = p.whole % pairs;
+    for (int i = 0; i < p.both; ++i)
+        if (p.parts > 1 && p.tma_out && p.out_type != T_F32 && (rc = result_map(&p.narrow[i], p.out_type, p.outp[i], p.M, p.N, p.ldo, 64))) return rc;
     for (int i = 0; i <= p.parts; ++i) p.share[i] = (int)((int64_t)p.chunks * i / p.parts);
     ProfScope prof_(c, c->stream, name);
     cudaLaunchAttribute at[2];
