@@ -589,15 +589,16 @@ int pair_clusters(dnb_ctx* c, int parts) {
     return n;
 }
 // Pairs a cluster and how many tiles are not split.  A tile costs its chunks of K and about four more; a split one a part of the chunks and about
-// ten (shares written, the cluster waited for, sums read).  us a call without / with: dx of 256 tokens, 2048 -> 5632 (8 tiles of 176 chunks) 65 / 31, of
-// 1024 tokens 66 / 43; 4-bit 512 tokens, 12288 -> 4096 (32 tiles of 48) 23.8 / 18; gated 512 tokens, 2560 -> 9728 in fp16 (152 tiles of 40) 48.4 / 46.
+// fourteen (shares written, the cluster waited for, sums read).  us a call without / with: dx of 256 tokens, 2048 -> 5632 (8 tiles of 176 chunks) 65 / 31, of
+// 1024 tokens 66 / 43; 4-bit 512 tokens, 12288 -> 4096 (32 tiles of 48) 23.8 / 18; gated 512 tokens, 2560 -> 9728 in fp16 (152 tiles of 40) 48.4 / 43;
+// 4-bit 256 tokens, 4096 -> 4096 (16 tiles of 16) 10.2 / 10.9, gated 1024 tokens, 1024 -> 2560 (80 tiles of 16) 15.2 / 16.8.
 template <class C>
 void choose_parts(dnb_ctx* c, int tiles, int chunks, int& parts, int& whole, int& clusters) {
     float least = 0.f;
     for (int s = 1; s <= 4; ++s) {
         const int n = pair_clusters<C>(c, s), turns = tiles / (n * s), rest = tiles - turns * n * s;
         const bool split = s > 1 && rest > 0 && rest <= n && chunks >= s;
-        const float cost = turns * (chunks + 4.f) + (rest == 0 ? 0.f : split ? (float)((chunks + s - 1) / s) + 10.f : chunks + 4.f);
+        const float cost = turns * (chunks + 4.f) + (rest == 0 ? 0.f : split ? (float)((chunks + s - 1) / s) + 14.f : chunks + 4.f);
         if (s == 1 || cost < least) least = cost, parts = s, whole = split ? turns * n * s : tiles, clusters = n;
     }
 }
