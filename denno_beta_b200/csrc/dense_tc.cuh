@@ -80,14 +80,32 @@ struct Cfg {
     static_assert(!FP4 || !AMN, "4-bit operands lie along K");
 };
 
-// Both activations are g / (1 + exp(-z)) with z = g (c0 + c1 g^2): silu has z = g, and v / 2 (1 + tanh(y)) = v / (1 + exp(-2 y)).  No branch,
-// two special functions; the approximate exponential and quotient are off by a few steps of 32 bits.
-struct ActForm { float c0, c1; };
+// Both activations are g / (1 + exp(-z)) with z = g (c0 + c1 g^2): silu has z = g, and v / 2 (1 + tanh(y)) = v / (1 + exp(-2 y)).  z has g's sign, so with
+// e = exp(-|z|) = h^2, h = 2^(-|z| / (2 ln 2)), it is g / (1 + e), or (g / (1 + e)) h h where g is negative: the divisor is in [1, 2], and h is a normal
+// number as far as h^2 is any, so that the two approximate instructions need no care for their ranges and results are right relative to their own size
+// down to the least numbers.  (exp(-z) in the divisor made zeros of results below 1e-36.)  Off by 7.5 steps of 2^-23, and by |z| of them for the
+// rounding of h's argument, as a rounding of g would cause.  expf(-|z|) was 8 to 27 % slower a call in 4-bit gated products of 256 to 4096 in K.
+struct ActForm { float c0, c1; };  // over 2 ln 2
+constexpr float kTwoLn2 = 1.3862943611198906f;
 __device__ __forceinline__ ActForm act_form(int act) {
-    return act == ACT_SILU ? ActForm{1.f, 0.f} : ActForm{1.5957691216057308f, 1.5957691216057308f * 0.044715f};
+    constexpr float silu = 1.f / kTwoLn2, gelu = 1.5957691216057308f / kTwoLn2;
+    return act == ACT_SILU ? ActForm{silu, 0.f} : ActForm{gelu, gelu * 0.044715f};
 }
 __device__ __forceinline__ float act_square(float g) { return fminf(g * g, 1e30f); }  // finite, so that 0 times it is 0
-__device__ __forceinline__ float act_of(ActForm f, float g) { return __fdividef(g, 1.f + __expf(-g * fmaf(f.c1, act_square(g), f.c0))); }
+__device__ __forceinline__ float power_of_two(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float act_of(ActForm f, float g) {
+    const float h = power_of_two(-fabsf(g * fmaf(f.c1, act_square(g), f.c0))), q = g * reciprocal(fmaf(h, h, 1.f)), s = g < 0.f ? h : 1.f;
+    return q * s * s;
+}
 
 template <int OUT>
 __device__ __forceinline__ void put(void* out, size_t at, float v) {

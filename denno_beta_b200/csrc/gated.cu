@@ -16,11 +16,12 @@ using namespace dt;
 using dt::Cfg;
 using dt::Params;
 
-// With p = 1 / (1 + exp(-z)): act = g p, act' = p + g p (1 - p) z'.
+// With p = 1 / (1 + exp(-z)): act = g p, act' = p + g p (1 - p) z'.  p and 1 - p from h (act_of), so that neither cancels nor vanishes.
 __device__ __forceinline__ void act_and_slope(ActForm f, float g, float& a, float& slope) {
-    const float s = act_square(g), p = __fdividef(1.f, 1.f + __expf(-g * fmaf(f.c1, s, f.c0)));
+    const float s = act_square(g), h = power_of_two(-fabsf(g * fmaf(f.c1, s, f.c0))), big = reciprocal(fmaf(h, h, 1.f)), small = big * h * h;
+    const float p = g < 0.f ? small : big, rest = g < 0.f ? big : small;
     a = g * p;
-    slope = p + a * (1.f - p) * fmaf(3.f * f.c1, s, f.c0);
+    slope = fmaf(a * rest, fmaf(3.f * f.c1, s, f.c0) * kTwoLn2, p);
 }
 
 // Eight features a thread: pre [2][nt][n] fp32, dout rows ldd apart, dpre [2][nt][n].  Memory: 4096 x 10240 in bf16, 587 MB, 84 us
