@@ -571,38 +571,6 @@ cudaLaunchConfig_t pair_config(dnb_ctx* c, cudaLaunchAttribute (&at)[2], unsigne
     cfg.numAttrs = 2;
     return cfg;
 }
-// Clusters of `parts` pairs that the device holds at once (GPCs leave some SMs over).  Asked once a device.
-template <class C>
-int pair_clusters(dnb_ctx* c, int parts) {
-    static std::atomic<int> known[64][5];
-    std::atomic<int>& k = known[c->device & 63][parts];
-    int n = k.load(std::memory_order_relaxed);
-    if (n == 0) {
-        cudaLaunchAttribute at[2];
-        const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2 * parts, parts);
-        if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<C>, &cfg) != cudaSuccess || n < 1) {
-            cudaGetLastError();
-            n = 1;
-        }
-        k.store(n, std::memory_order_relaxed);
-    }
-    return n;
-}
-// Pairs a cluster and how many tiles are not split.  A tile costs its chunks of K and about four more; a split one a part of the chunks and about
-// fourteen (shares written, the cluster waited for, sums read).  us a call without / with: dx of 256 tokens, 2048 -> 5632 (8 tiles of 176 chunks) 65 / 31, of
-// 1024 tokens 66 / 43; 4-bit 512 tokens, 12288 -> 4096 (32 tiles of 48) 23.8 / 18; gated 512 tokens, 2560 -> 9728 in fp16 (152 tiles of 40) 48.4 / 43;
-// 4-bit 256 tokens, 4096 -> 4096 (16 tiles of 16) 10.2 / 10.9, gated 1024 tokens, 1024 -> 2560 (80 tiles of 16) 15.2 / 16.8.
-template <class C>
-void choose_parts(dnb_ctx* c, int tiles, int chunks, int& parts, int& whole, int& clusters) {
-    float least = 0.f;
-    for (int s = 1; s <= 4; ++s) {
-        const int n = pair_clusters<C>(c, s), turns = tiles / (n * s), rest = tiles - turns * n * s;
-        const bool split = s > 1 && rest > 0 && rest <= n && chunks >= s;
-        const float cost = turns * (chunks + 4.f) + (rest == 0 ? 0.f : split ? (float)((chunks + s - 1) / s) + 14.f : chunks + 4.f);
-        if (s == 1 || cost < least) least = cost, parts = s, whole = split ? turns * n * s : tiles, clusters = n;
-    }
-}
-
 // p: M, N, K, passes, both, type, act, outp, out_scales, ldo; maps of scales and pre where there are any.
 template <class C>
 int launch_pair(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* b, int nb, int type, const char* name) {
@@ -634,17 +602,21 @@ int launch_pair(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand* 
     p.last_group = divisor(p.tiles_m % 8 ? p.tiles_m % 8 : 8);
     static SmemGrant grant;
     DNB_CUDA(grant_smem(grant, c->device, pair_kernel<C>, C::SMEM));
-    int clusters;
-    choose_parts<C>(c, p.tiles, p.chunks, p.parts, p.whole, clusters);
-    const int used = p.parts > 1 && p.whole > 0 ? clusters : p.tiles < clusters ? p.tiles : clusters, pairs = used * p.parts;
-    p.each = p.whole / pairs;
-    p.more = p.whole % pairs;
+    static std::atomic<int> known[64][5];
+    int at_once[5];
+    cudaLaunchAttribute at[2];
+    for (int s = 1; s <= 4; ++s) at_once[s] = clusters_at_once(known[c->device][s], pair_kernel<C>, pair_config<C>(c, at, 2 * s, s));
+    if (at_once[1] < 1) at_once[1] = 1;  // one pair takes the tiles in turn, if any can be launched
+    const PairPlan plan = pair_plan(at_once, p.tiles, p.chunks);
+    p.parts = plan.parts;
+    p.whole = plan.whole;
+    p.each = plan.each;
+    p.more = plan.more;
     for (int i = 0; i < p.both; ++i)
         if (p.parts > 1 && p.tma_out && p.out_type != T_F32 && (rc = result_map(&p.narrow[i], p.out_type, p.outp[i], p.M, p.N, p.ldo, 64))) return rc;
     for (int i = 0; i <= p.parts; ++i) p.share[i] = (int)((int64_t)p.chunks * i / p.parts);
     ProfScope prof_(c, c->stream, name);
-    cudaLaunchAttribute at[2];
-    const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2u * (unsigned)pairs, p.parts);
+    const cudaLaunchConfig_t cfg = pair_config<C>(c, at, 2u * (unsigned)plan.pairs, p.parts);
     DNB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<C>, p));
     c->launches++;
     return DNB_OK;

@@ -21,6 +21,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include "dense_plan.h"
 #include "dnb_common.cuh"
 #include "tc_ptx.cuh"
 #include "tensor_map.cuh"
@@ -532,42 +533,19 @@ cudaLaunchConfig_t launch_config(dnb_ctx* c, cudaLaunchAttribute (&at)[2], unsig
     return cfg;
 }
 
-// How many clusters of `splits` blocks the device holds at once: blocks of a cluster share a GPC, whose SMs they may not fill (15 clusters of eight
-// blocks that each want an SM, where 148 SMs could hold 18).  Asked once a device.
-template <class C>
-int clusters_at_once(dnb_ctx* c, int splits) {
-    static std::atomic<int> known[64][9];
-    std::atomic<int>& k = known[c->device & 63][splits];
-    int n = k.load(std::memory_order_relaxed);
+// How many clusters the device holds at once, 0: none, or it did not say (which is asked again).  Blocks of a cluster share a GPC, whose SMs they may not
+// fill (15 clusters of eight blocks that each want an SM, where 148 SMs could hold 18).  Asked once a device.
+template <class K>
+int clusters_at_once(std::atomic<int>& known, K kernel, const cudaLaunchConfig_t& cfg) {
+    int n = known.load(std::memory_order_relaxed);
     if (n == 0) {
-        cudaLaunchAttribute at[2];
-        cudaLaunchConfig_t cfg = launch_config<C>(c, at, splits, splits);
-        if (splits == 1) n = c->sm_count * C::PER_SM;
-        else if (cudaOccupancyMaxActiveClusters(&n, dense_kernel<C>, &cfg) != cudaSuccess || n < 1) {
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
             cudaGetLastError();
-            n = 1;
+            return 0;
         }
-        k.store(n, std::memory_order_relaxed);
+        known.store(n > 0 ? n : -1, std::memory_order_relaxed);
     }
-    return n;
-}
-
-// Into how many parts K is split.  A block costs its chunks of K and, in chunks, what starting and joining it takes (about 100 KB of weights' time);
-// a second block on an SM costs 0.85 of another turn, as an SM's share of the memory's rate is nearly that of one block; another wave costs a whole
-// turn.  us a call for 1 to 8 parts: 4 tokens, 4096 -> 10240 gated in bf16 (80 tiles) 36, 39, 33, 39, 35, 35, 40, 38; dx of 77 tokens (17 tiles, one
-// block an SM) - , -, 32, 28, 25, 24, 36, 34 (beyond 6 parts the clusters take two waves); 4-bit 12288 -> 4096 (32 tiles) -, -, 9.7, 8.5, 8.6, 8.3, 7.8, 7.6.
-template <class C>
-int best_splits(dnb_ctx* c, int tiles, int chunks) {
-    const float start = 100.f * 1024.f / C::STAGE;
-    int best = 1;
-    float least = 0.f;
-    for (int s = 1; s <= 8 && s <= chunks; ++s) {
-        const int at_once = clusters_at_once<C>(c, s), waves = (tiles + at_once - 1) / at_once, blocks = (tiles < at_once ? tiles : at_once) * s;
-        const float turns = 1.f + 0.85f * ((blocks + c->sm_count - 1) / c->sm_count - 1);
-        const float cost = waves * (start + (chunks + s - 1) / s * turns) + 0.15f * s;
-        if (s == 1 || cost < least) best = s, least = cost;
-    }
-    return best;
+    return n > 0 ? n : 0;
 }
 
 // p: everything but the maps, the operands' type and the splits.  a, b: C::NA or p.passes operands of A, p.passes of B.
@@ -585,13 +563,16 @@ int launch_dense(dnb_ctx* c, Params& p, const Operand* a, int na, const Operand*
     static_assert(C::ACC * TM * 4 <= C::STAGES * C::STAGE, "the partial sums of a split lie in the ring");
     static SmemGrant grant;
     DNB_CUDA(grant_smem(grant, c->device, dense_kernel<C>, C::SMEM));
-    p.splits = best_splits<C>(c, tiles, chunks);
+    static std::atomic<int> known[64][9];
+    int at_once[9] = {0, c->sm_count * C::PER_SM};
+    cudaLaunchAttribute at[2];
+    for (int s = 2; s <= 8 && s <= chunks; ++s) at_once[s] = clusters_at_once(known[c->device][s], dense_kernel<C>, launch_config<C>(c, at, s, s));
+    p.splits = best_splits(at_once, c->sm_count, C::STAGE, tiles, chunks);
     p.chunks = chunks;
     for (int i = 0; i <= p.splits; ++i) p.share[i] = (int)((int64_t)chunks * i / p.splits);
     const int slots = c->sm_count * C::PER_SM;
     const unsigned grid = p.splits > 1 ? (unsigned)tiles * p.splits : (unsigned)(tiles < slots ? tiles : slots);
     ProfScope prof_(c, c->stream, name);
-    cudaLaunchAttribute at[2];
     const cudaLaunchConfig_t cfg = launch_config<C>(c, at, grid, p.splits);
     DNB_CUDA(cudaLaunchKernelEx(&cfg, dense_kernel<C>, p));
     c->launches++;
