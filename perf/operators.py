@@ -174,17 +174,20 @@ def prepare(case, seed):
 
 # ---- a pass ------------------------------------------------------------------------------------------------------------------
 
-_contexts = []
+_contexts = {}
 
 
 def _context():
-    """The framework's context of this process, on the stream that torch works on."""
-    from denno_beta_b200 import cuda as cu
-    if not _contexts:
-        c = cu.CudaCtx(torch.cuda.current_device())
-        c.set_stream(torch.cuda.current_stream().cuda_stream or 1)  # 1: the default stream by its handle
-        _contexts.append(c)
-    return cu, _contexts[0]
+    """The framework and its context for the current device and the stream that torch works on there, now: a context works on one stream.
+    Asked by torch's raw calls: a Stream object takes as long as a small call."""
+    device = torch._C._cuda_getDevice()
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    found = _contexts.get((device, stream))
+    if found is None:
+        from denno_beta_b200 import cuda as cu
+        found = _contexts[device, stream] = cu, cu.CudaCtx(device)
+        found[1].set_stream(stream or 1)  # 1: the default stream by its handle
+    return found
 
 
 def _done(ok):
