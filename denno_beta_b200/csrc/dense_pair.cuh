@@ -533,7 +533,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) pair_kernel(const __grid_cons
         if (lane == 0) store_read<0>();  // the boxes have been read
     }
     __syncwarp();
-    __syncwarp();
     tc_fence_before();
     // Nobody's shared or tensor memory goes while another may still use it: reads are over, and every arrival at another CTA's barrier has been waited for.
     cluster_leave();

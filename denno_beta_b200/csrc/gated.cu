@@ -33,29 +33,29 @@ gradients_kernel(int act_id, const float* __restrict__ pre, const void* __restri
     pdl_launch_dependents();
     const ActForm act = act_form(act_id);
     const size_t per = n / 8, all = per * nt, plane = (size_t)nt * n;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
-        const size_t t = i / per, at = (i - t * per) * 8;
-        float g[8], u[8];
-        const float4* gp = reinterpret_cast<const float4*>(pre + t * n + at);
-        const float4* up = reinterpret_cast<const float4*>(pre + plane + t * n + at);
-        *reinterpret_cast<float4*>(g) = gp[0];
-        *reinterpret_cast<float4*>(g + 4) = gp[1];
-        *reinterpret_cast<float4*>(u) = up[0];
-        *reinterpret_cast<float4*>(u + 4) = up[1];
-        const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dout) + t * ldd + at);
-        uint4 og, ou;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= all) return;
+    const size_t t = i / per, at = (i - t * per) * 8;
+    float g[8], u[8];
+    const float4* gp = reinterpret_cast<const float4*>(pre + t * n + at);
+    const float4* up = reinterpret_cast<const float4*>(pre + plane + t * n + at);
+    *reinterpret_cast<float4*>(g) = gp[0];
+    *reinterpret_cast<float4*>(g + 4) = gp[1];
+    *reinterpret_cast<float4*>(u) = up[0];
+    *reinterpret_cast<float4*>(u + 4) = up[1];
+    const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dout) + t * ldd + at);
+    uint4 og, ou;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint16_t b = reinterpret_cast<const uint16_t*>(&raw)[j];
-            const float d = T == T_BF16 ? __bfloat162float(__ushort_as_bfloat16(b)) : __half2float(__ushort_as_half(b));
-            float a, slope;
-            act_and_slope(act, g[j], a, slope);
-            put<T>(&og, j, d * u[j] * slope);
-            put<T>(&ou, j, d * a);
-        }
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dpre) + t * n + at) = og;
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dpre) + plane + t * n + at) = ou;
+    for (int j = 0; j < 8; ++j) {
+        const uint16_t b = reinterpret_cast<const uint16_t*>(&raw)[j];
+        const float d = T == T_BF16 ? __bfloat162float(__ushort_as_bfloat16(b)) : __half2float(__ushort_as_half(b));
+        float a, slope;
+        act_and_slope(act, g[j], a, slope);
+        put<T>(&og, j, d * u[j] * slope);
+        put<T>(&ou, j, d * a);
     }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dpre) + t * n + at) = og;
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dpre) + plane + t * n + at) = ou;
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -144,6 +144,11 @@ int dnb_gated_backward_dev(dnb_ctx* c, int act, int type, const void* x_dev, siz
     if (!c) return DNB_ERR_ARG;
     int rc = check_shape("gated_backward", act, type, nt, k, n);
     if (rc) return rc;
+    const size_t blocks = ((size_t)nt * n / 8 + 255) / 256;
+    if (blocks > 0x7fffffff) {
+        set_error("gated_backward: %d x %d is more than one launch takes", nt, n);
+        return DNB_DECLINED;
+    }
     const bool weights = dgate_dev || dup_dev;
     if (weights && (!dgate_dev || !dup_dev)) {
         set_error("gated_backward: gradients of both weights, or of none");
@@ -172,10 +177,9 @@ int dnb_gated_backward_dev(dnb_ctx* c, int act, int type, const void* x_dev, siz
         }
         return DNB_OK;
     }
-    const size_t groups = (size_t)nt * n / 8, want = (groups + 255) / 256, most = 0x7fffffff;
     {
         ProfScope prof_(c, c->stream, "gated_gradients");
-        const dim3 grid((unsigned)(want < most ? want : most));
+        const dim3 grid((unsigned)blocks);
         if (type == T_BF16) DNB_CUDA(launch_k(gradients_kernel<T_BF16>, grid, dim3(256), 0, c->stream, c->use_pdl, act, pre_dev, dout_dev, ldd, nt, n, dpre_dev));
         else DNB_CUDA(launch_k(gradients_kernel<T_F16>, grid, dim3(256), 0, c->stream, c->use_pdl, act, pre_dev, dout_dev, ldd, nt, n, dpre_dev));
         c->launches++;

@@ -18,20 +18,15 @@ using dt::Params;
 // divisions and a branch at each load, which waited for it: 47 and 37).
 constexpr int THREADS = 256, UNITS = THREADS / 16;
 
-// Where a thread is: unit u = folded row * nkb + kb, a folded row being 32 * tile + r.  Advanced without a division.
+// Where a thread is: unit u = folded row * nkb + kb, a folded row being 32 * tile + r.  Advanced without a division.  Fewer than 2^31 units (check_units).
 struct Walk {
     size_t u, units, row;  // row: the first of the four
     int kb, nkb, dkb;
     size_t dq, q;
     __device__ Walk(size_t folded, int nkb_) : units(folded * nkb_), nkb(nkb_) {
-        u = (size_t)blockIdx.x * UNITS + (threadIdx.x >> 4);
-        const size_t step = (size_t)gridDim.x * UNITS;
-        if (units >> 31) {
-            q = u / nkb; kb = (int)(u - q * nkb); dq = step / nkb; dkb = (int)(step - dq * nkb);
-        } else {
-            const uint32_t qs = (uint32_t)u / (uint32_t)nkb, ds = (uint32_t)step / (uint32_t)nkb;
-            q = qs; kb = (int)((uint32_t)u - qs * nkb); dq = ds; dkb = (int)((uint32_t)step - ds * nkb);
-        }
+        const uint32_t start = blockIdx.x * UNITS + (threadIdx.x >> 4), step = gridDim.x * UNITS, qs = start / (uint32_t)nkb, ds = step / (uint32_t)nkb;
+        u = start;
+        q = qs; kb = (int)(start - qs * nkb); dq = ds; dkb = (int)(step - ds * nkb);
         place();
     }
     __device__ void place() { row = (q >> 5) * 128 + (q & 31); }
@@ -295,6 +290,13 @@ static int check_sizes(const char* what, int nt, int k, int n) {
     return DNB_DECLINED;
 }
 
+// Units that Walk counts: a launch's worth of rows (half a terabyte of codes and more).
+static int check_units(const char* what, int rows, int k) {
+    if (folded_rows(rows) * (size_t)((k - 1) / 128 + 1) < (size_t)1 << 31) return DNB_OK;
+    set_error("%s: %d rows of %d are more than one launch takes", what, rows, k);
+    return DNB_DECLINED;
+}
+
 // One product (NA 1) or the gated one (2).  Up to 128 tokens: narrow tiles of tokens under the weights' rows (dense_tc.cuh); beyond, tiles of
 // 256 tokens (dense_pair.cuh).
 template <int NA>
@@ -364,7 +366,7 @@ int dnb_mx4_quantize_dev(dnb_ctx* c, int type, const void* x_dev, size_t ldx, in
         set_error("mx4_quantize: rows of ggml type %d, %zu elements apart, are not handled", type, ldx);
         return DNB_DECLINED;
     }
-    if (rows == 0) return DNB_OK;
+    if ((rc = check_units("mx4_quantize", rows, k)) || rows == 0) return rc;
     DNB_CUDA(cudaSetDevice(c->device));
     const int nkb = (k + 127) / 128;
     const size_t folded = folded_rows(rows);
@@ -394,7 +396,7 @@ int dnb_mx4_dequantize_dev(dnb_ctx* c, const void* codes_dev, const void* scales
         set_error("mx4_dequantize: results of ggml type %d are not handled", type);
         return DNB_DECLINED;
     }
-    if (rows == 0) return DNB_OK;
+    if ((rc = check_units("mx4_dequantize", rows, k)) || rows == 0) return rc;
     DNB_CUDA(cudaSetDevice(c->device));
     const int nkb = (k + 127) / 128;
     const size_t folded = folded_rows(rows);
