@@ -20,19 +20,19 @@ constexpr int THREADS = 256, UNITS = THREADS / 16;
 
 // Where a thread is: unit u = folded row * nkb + kb, a folded row being 32 * tile + r.  Advanced without a division.  Fewer than 2^31 units (check_units).
 struct Walk {
-    size_t u, units, row;  // row: the first of the four
+    uint32_t u, units;
+    size_t row;  // the first of the four
     int kb, nkb, dkb;
-    size_t dq, q;
-    __device__ Walk(size_t folded, int nkb_) : units(folded * nkb_), nkb(nkb_) {
-        const uint32_t start = blockIdx.x * UNITS + (threadIdx.x >> 4), step = gridDim.x * UNITS, qs = start / (uint32_t)nkb, ds = step / (uint32_t)nkb;
-        u = start;
-        q = qs; kb = (int)(start - qs * nkb); dq = ds; dkb = (int)(step - ds * nkb);
+    uint32_t dq, q;
+    __device__ Walk(uint32_t folded, int nkb_) : u(blockIdx.x * UNITS + (threadIdx.x >> 4)), units(folded * nkb_), nkb(nkb_) {
+        const uint32_t step = gridDim.x * UNITS;
+        q = u / (uint32_t)nkb; kb = (int)(u - q * nkb); dq = step / (uint32_t)nkb; dkb = (int)(step - dq * nkb);
         place();
     }
-    __device__ void place() { row = (q >> 5) * 128 + (q & 31); }
+    __device__ void place() { row = (size_t)(q >> 5) * 128 + (q & 31); }
     __device__ bool warp_in() const { return u - ((threadIdx.x >> 4) & 1) < units; }  // the first of the warp's two units
     __device__ void next() {
-        u += (size_t)gridDim.x * UNITS;
+        u += gridDim.x * UNITS;
         q += dq;
         kb += dkb;
         if (kb >= nkb) kb -= nkb, ++q;
@@ -132,7 +132,7 @@ __device__ __forceinline__ void file_piece(const uint8_t* b, int at, uint32_t& c
 
 template <int T, bool WHOLE>
 __global__ void __launch_bounds__(THREADS)
-quantize_kernel(const void* __restrict__ x, size_t ldx, int rows, size_t folded, int k, int nkb, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+quantize_kernel(const void* __restrict__ x, size_t ldx, int rows, uint32_t folded, int k, int nkb, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 15;
@@ -202,7 +202,7 @@ __device__ __forceinline__ void four_values(uint32_t code, float s, float (&v)[4
 // 16 bytes of results a store, neighbouring lanes next to each other: 8 elements a lane, or (F32) 4 of each half of the 128 columns.
 template <int T, bool WHOLE>
 __global__ void __launch_bounds__(THREADS)
-dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, size_t folded, int k, int nkb, void* __restrict__ out, size_t ldo) {
+dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, uint32_t folded, int k, int nkb, void* __restrict__ out, size_t ldo) {
     pdl_wait();
     pdl_launch_dependents();
     using N = typename Num<T>::type;
