@@ -39,6 +39,7 @@ struct Walk {
         place();
     }
 };
+static int tiles_along(int k) { return (k - 1) / 128 + 1; }  // of scales
 static size_t folded_rows(int rows) { return (size_t)(rows / 128) * 32 + (rows % 128 < 32 ? rows % 128 : 32); }
 
 template <int T> struct Num { using type = float; };
@@ -292,7 +293,7 @@ static int check_sizes(const char* what, int nt, int k, int n) {
 
 // Units that Walk counts: a launch's worth of rows (half a terabyte of codes and more).
 static int check_units(const char* what, int rows, int k) {
-    if (folded_rows(rows) * (size_t)((k - 1) / 128 + 1) < (size_t)1 << 31) return DNB_OK;
+    if (folded_rows(rows) * tiles_along(k) < (size_t)1 << 31) return DNB_OK;
     set_error("%s: %d rows of %d are more than one launch takes", what, rows, k);
     return DNB_DECLINED;
 }
@@ -349,7 +350,7 @@ int dnb_mx4_bytes(int rows, int k, size_t* codes, size_t* scales) {
         return DNB_DECLINED;
     }
     *codes = (size_t)rows * k / 2;
-    *scales = ((size_t)rows + 127) / 128 * ((k + 127) / 128) * 512;
+    *scales = ((size_t)rows + 127) / 128 * tiles_along(k) * 512;
     return DNB_OK;
 }
 
@@ -368,7 +369,7 @@ int dnb_mx4_quantize_dev(dnb_ctx* c, int type, const void* x_dev, size_t ldx, in
     }
     if ((rc = check_units("mx4_quantize", rows, k)) || rows == 0) return rc;
     DNB_CUDA(cudaSetDevice(c->device));
-    const int nkb = (k + 127) / 128;
+    const int nkb = tiles_along(k);
     const size_t folded = folded_rows(rows);
     const dim3 grid(grid_of(c, folded * nkb, TO_FOUR_BITS)), block(THREADS);
     const bool whole = aligned16(x_dev) && ldx * es % 16 == 0;
@@ -398,7 +399,7 @@ int dnb_mx4_dequantize_dev(dnb_ctx* c, const void* codes_dev, const void* scales
     }
     if ((rc = check_units("mx4_dequantize", rows, k)) || rows == 0) return rc;
     DNB_CUDA(cudaSetDevice(c->device));
-    const int nkb = (k + 127) / 128;
+    const int nkb = tiles_along(k);
     const size_t folded = folded_rows(rows);
     const dim3 grid(grid_of(c, folded * nkb, BACK)), block(THREADS);
     const bool whole = aligned16(out_dev) && ldo * es % 16 == 0;
