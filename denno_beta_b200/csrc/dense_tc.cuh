@@ -34,6 +34,8 @@ constexpr int TM = 128;             // rows of A in a tile
 constexpr int NTHREADS = 320;
 constexpr int EPI_WARPS = 8;
 constexpr int kWaitStage = 27, kWaitAcc = 28, kWaitDrain = 29;  // status codes of the waits
+// Chunks of K of the longest sum.  A tile's results are waited for while its sum runs, 0.3 to 0.7 us a chunk, and a wait gives up after half a second.
+constexpr int kMostChunks = 1 << 19;
 
 enum Act { ACT_NONE = -1, ACT_SILU = 0, ACT_GELU = 1 };
 

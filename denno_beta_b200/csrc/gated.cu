@@ -72,6 +72,12 @@ static int check_shape(const char* what, int act, int type, int nt, int k, int n
     }
     return DNB_OK;
 }
+// A sum that a wait outlasts (64 a chunk).
+static int check_sum(const char* what, const char* over, int64_t terms) {
+    if (terms <= (int64_t)kMostChunks * 64) return DNB_OK;
+    set_error("%s: a sum over %lld %s is more than one launch takes (2^25)", what, (long long)terms, over);
+    return DNB_DECLINED;
+}
 // Rows of a matrix that TMA or 16-byte loads take.
 static int check_rows(const char* what, const char* name, const void* p, size_t ld, int cols) {
     if (!p || ld < (size_t)cols) {
@@ -97,7 +103,7 @@ int dnb_gated_dev(dnb_ctx* c, int act, int type, const void* x_dev, size_t ldx, 
                   size_t ldo, float* pre_dev) {
     if (!c) return DNB_ERR_ARG;
     int rc = check_shape("gated", act, type, nt, k, n);
-    if (rc || nt == 0) return rc;
+    if (rc || (rc = check_sum("gated", "elements of a row", k)) || nt == 0) return rc;
     if ((rc = check_rows("gated", "x", x_dev, ldx, k))) return rc;
     if ((rc = check_rows("gated", "gate", gate_dev, k, k))) return rc;
     if ((rc = check_rows("gated", "up", up_dev, k, k))) return rc;
@@ -154,6 +160,8 @@ int dnb_gated_backward_dev(dnb_ctx* c, int act, int type, const void* x_dev, siz
         set_error("gated_backward: gradients of both weights, or of none");
         return DNB_ERR_ARG;
     }
+    if (dx_dev && (rc = check_sum("gated_backward", "features of gate and up", 2 * (int64_t)n))) return rc;
+    if (weights && (rc = check_sum("gated_backward", "tokens", nt))) return rc;
     if ((uintptr_t)dgate_dev % 2 || (uintptr_t)dup_dev % 2 || (uintptr_t)dx_dev % 2) {
         set_error("gated_backward: misaligned result");
         return DNB_DECLINED;

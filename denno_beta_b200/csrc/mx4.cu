@@ -284,10 +284,10 @@ static int check_matrix(const char* what, const void* codes, const void* scales,
     return DNB_OK;
 }
 
-// Sizes that tiles are counted for in 32 bits.
+// Sizes that tiles are counted for in 32 bits, and sums that a wait outlasts.
 static int check_sizes(const char* what, int nt, int k, int n) {
-    if (nt <= 1 << 30 && k <= 1 << 30 && n <= 1 << 30) return DNB_OK;
-    set_error("%s: %d x %d x %d is more than one launch takes", what, nt, k, n);
+    if (nt <= 1 << 30 && k <= kMostChunks * 256 && n <= 1 << 30) return DNB_OK;
+    set_error("%s: %d x %d x %d is more than one launch takes (k up to 2^27)", what, nt, k, n);
     return DNB_DECLINED;
 }
 

@@ -189,7 +189,8 @@ int dnb_set_router_tc(dnb_ctx* ctx, int on);
  *     Of a tile that reaches beyond the matrix, scales past a row's end are zero; rows past the last are never looked at.
  * All pointers are device pointers of the context's device; the calls are asynchronous on the context's stream, allocate
  * nothing and keep nothing, so that they can be captured into a graph.  Results must not overlap operands.  No tokens
- * (rows, nt = 0) is DNB_OK and does nothing.  DNB_DECLINED: a type, k or alignment that the kernels do not take.
+ * (rows, nt = 0) is DNB_OK and does nothing.  DNB_DECLINED: a type, k or alignment that the kernels do not take, or a size that
+ * one launch does not (nt or n beyond 2^30, k of a product beyond 2^27).
  *   dnb_mx4_bytes: how long the two arrays are.
  *   dnb_mx4_quantize_dev: rows of F32, F16 or BF16, ldx elements apart (aligned as their type), to such a matrix.  The scale's
  *       exponent is floor(log2(largest magnitude of the 32)) - 2, at least -127; elements are rounded to nearest, ties to
@@ -219,6 +220,7 @@ int dnb_mx4_gated_dev(dnb_ctx* ctx, int act, const void* x_codes, const void* x_
  * moe_expert.rs silu(gate x) * up x) and its gradients.  type: F16 or BF16, of all operands and results but pre (fp32).
  * x [nt][k], gate and up [n][k]; k and n multiples of 8; rows of x, dout ldx, ldd (multiples of 8) elements apart, of out and
  * dx ldo, lddx; operands and pre, dpre start at multiples of 16 bytes.  Device pointers, asynchronous, nothing allocated, as above.
+ * Sizes up to 2^30, and sums of up to 2^25 terms: k in the forward pass, 2 n for dx, nt for the weights' gradients.
  *   dnb_gated_dev: g = x gate^T, u = x up^T, out = act(g) * u.  pre (NULL without a backward pass): [2][nt][n], g and then u.
  *   dnb_gated_backward_dev: from pre and dout [nt][n], the gradient of out:
  *       dpre [2][nt][n]: dout * u * act'(g) and dout * act(g), rounded to the type (wanted in any case: the operands of the rest),
