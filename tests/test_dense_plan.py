@@ -67,3 +67,22 @@ def test_clusters_that_a_device_does_not_hold_are_not_used(plan):
     for tiles, chunks, none in itertools.product([1, 17, 80, 500], [1, 3, 8, 16, 48], itertools.combinations(range(2, 9), 3)):
         s = plan.splits(held(*none), 148, 20480, tiles, chunks)
         assert 1 <= s <= min(8, chunks) and s not in none
+
+
+def test_sizes_that_are_tested_take_the_paths_they_are_for(plan):
+    """On any device with about a B200's clusters, whatever a change of the rules makes of them."""
+    import dense_sizes as sizes
+
+    for (nt, k, n), columns in [*((s, 256) for s in sizes.SPLIT_PRODUCTS), *((s, 128) for s in sizes.SPLIT_GATED)]:
+        tiles = -(-nt // 256) * -(-n // columns)
+        for at_once in ([0, *c] for c in itertools.product((70, 72, 74), (33, 35, 37), (20, 22, 24), (14, 16, 18))):
+            p = pairs(plan, at_once, tiles, -(-k // 256))
+            assert p["parts"] > 1 and p["whole"] < tiles and (p["whole"] > 0) == (tiles >= 74)
+    for gated, listed in ((0, sizes.SEVERAL_A_BLOCK_PRODUCTS), (1, sizes.SEVERAL_A_BLOCK_GATED)):
+        for nt, k, n in listed:
+            tiles, per_sm, rows = -(-n // 128), 2 if nt <= 64 else 1, next(r for r in (16, 32, 64, 128) if nt <= r)
+            assert tiles > 148 * per_sm
+            stage16 = (1 + gated) * 16384 + rows * 128
+            for stage, chunks in ((stage16 + (2 + gated) * 1024, -(-k // 256)), (stage16, -(-k // 64))):  # 4 bits, 16 bits
+                held = [0, 148 * per_sm, *((148 * per_sm - 8) // s for s in range(2, 9))]
+                assert plan.splits((C.c_int * 9)(*held), 148, stage, tiles, chunks) == 1
