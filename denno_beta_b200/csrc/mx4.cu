@@ -14,8 +14,9 @@ using dt::Params;
 
 // A thread takes 8 elements of the rows r, r + 32, r + 64 and r + 96 of a tile of scales, 16 threads (half a warp) its 128 columns: four independent
 // 16- or 32-byte loads in flight a thread, and the 16 bytes of scales that these rows have next to each other are one store.  A block of 32 is four
-// neighbouring lanes.  Bound by memory: 14018 x 4096, fp32 to 4 bits 40 us (6.5 TB/s), bf16 29 (5.0) and back 26 (5.6; a row a thread at a time, 64-bit
-// divisions and a branch at each load, which waited for it: 47 and 37).
+// neighbouring lanes.  Bound by memory: 14018 x 4096, fp32 to 4 bits 40 us (6.5 TB/s), bf16 26.1 (5.6) and back 23.5 (6.2; a row a thread at a time, 64-bit
+// divisions and a branch at each load, which waited for it: 47 and 37).  A file's blocks, whose 17 bytes start anywhere, 23 (2.6): nine
+// loads of a byte a piece bound it; weights go through it once, as they are loaded.
 constexpr int THREADS = 256, UNITS = THREADS / 16;
 
 // Where a thread is: unit u = folded row * nkb + kb, a folded row being 32 * tile + r.  Advanced without a division.  Fewer than 2^31 units (check_units).
@@ -255,9 +256,9 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     }
 }
 
-// Blocks an SM, more than fit at once (4 and 6), so that the SMs end together; us for 14018 x 4096 bf16 with 4, 8, 16, 48 an SM: to 4 bits 30.0, 28.9, 29.1,
-// 32.2, back 33.7, 28.8, 26.0, 26.9.
-constexpr int TO_FOUR_BITS = 8, BACK = 16;
+// Blocks an SM, more than fit at once (5 and 8), so that the SMs end together; us for 14018 x 4096 bf16 with 4, 8, 16, 48 an SM: to 4 bits 31.2, 26.7, 26.1,
+// 28.3, back 27.1, 27.7, 26.0, 23.5.
+constexpr int TO_FOUR_BITS = 16, BACK = 48;
 static unsigned grid_of(const dnb_ctx* c, size_t units, int an_sm) {
     const size_t want = (units + UNITS - 1) / UNITS, most = (size_t)c->sm_count * an_sm;
     return (unsigned)(want < most ? want : most);
