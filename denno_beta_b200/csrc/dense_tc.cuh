@@ -248,23 +248,26 @@ __device__ __forceinline__ void put4(void* out, size_t at, const float (&o)[4], 
     for (int i = 0; i < 4; ++i)
         if (i < left) put<OUT>(out, at + i, o[i]);
 }
-// The sums of columns' shares, in rank order: a warp two columns at a time, four neighbouring features a lane, all shares asked for at once.
+// The sums of columns' shares, in rank order: a warp two columns at a time, four neighbouring features a lane, all shares asked for at once.  One column where two
+// accumulators meet the 96 registers of two blocks an SM: with two, 588 bytes went to local memory (452 in 16 bits).  us a call with two / one: 4-bit gated 2048 -> 8192
+// of 1, 8, 33 tokens 5.3 / 4.9, 6.0 / 4.9, 7.8 / 6.8; bf16 gated 4 tokens, 4096 -> 10240 31.1 / 29.0, 64 tokens, 2048 -> 5632 18.0 / 16.2.
 template <class C, int OUT>
 __device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t red, uint32_t rank, int warp, int lane) {
     const int m = tile * TM + 4 * lane, left = p.M - m;
     const ActForm act = act_form(p.act);
     const bool whole = ((p.ldo | (reinterpret_cast<uintptr_t>(p.out) / (OUT == T_F32 ? 4 : 2))) & 3) == 0;
     const int step = EPI_WARPS * p.splits;
+    constexpr int COLUMNS = C::NA == 2 && C::PER_SM == 2 ? 1 : 2;
 #pragma unroll 1
-    for (int c0 = (int)rank + p.splits * warp; c0 < p.N; c0 += 2 * step) {
-        float4 s[2][C::NA];
+    for (int c0 = (int)rank + p.splits * warp; c0 < p.N; c0 += COLUMNS * step) {
+        float4 s[COLUMNS][C::NA];
         for (int r = 0; r < p.splits; r += 4) {
-            float4 v[2][C::NA][4];
+            float4 v[COLUMNS][C::NA][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (r + i < p.splits) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < COLUMNS; ++j)
 #pragma unroll
                         for (int a = 0; a < C::NA; ++a)  // a second column beyond the last reads where the ring was
                             v[j][a][i] = peer_floats(red + 4u * (uint32_t)((a * C::BN + min(c0 + j * step, C::BN - 1)) * TM + 4 * lane), r + i);
@@ -273,7 +276,7 @@ __device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t re
             for (int i = 0; i < 4; ++i)
                 if (r + i < p.splits) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < COLUMNS; ++j)
 #pragma unroll
                         for (int a = 0; a < C::NA; ++a) {
                             float4& d = s[j][a];
@@ -284,7 +287,7 @@ __device__ __forceinline__ void split_out(const Params& p, int tile, uint32_t re
                 }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < COLUMNS; ++j) {
             const int c = c0 + j * step;
             if (c >= p.N) break;
             float o[4] = {s[j][0].x, s[j][0].y, s[j][0].z, s[j][0].w};
