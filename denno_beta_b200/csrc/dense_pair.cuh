@@ -16,9 +16,10 @@
 //
 // What bounds it.  A chunk (64 of K in 16 bits, 256 in 4) takes 615 and 650 cycles where its MMAs alone take 512: the copies that come in and what the
 // MMAs read are 107 bytes a clock of shared memory's 128; the scales' way to tensor memory is 4 % of a chunk.  Two tiles that share a B (three quarters
-// of the copies) were 1.5 to 5 % faster on long runs, no faster on short ones, and are not kept.  Long runs are bound by the power limit: bf16 4096 tokens, 4096 -> 10240, 1.57 PFLOP/s for some milliseconds (0.93 of the measured
-// peak), 1.36 at 1.2 to 1.35 GHz; 4 bits, 8192 tokens, 4096 -> 8192, 104 us (5.3 PFLOP/s), 129 at 1.6 GHz.  Short ones: about 5 us of launch, set-up and
-// first copies, and a first tile's epilogue of 2,500 cycles (1,100 once its code is in the instruction cache).
+// of the copies) were 1.5 to 5 % faster on long runs, no faster on short ones, and are not kept.  Long runs are bound by the power limit: bf16 4096 tokens,
+// 4096 -> 10240, 1.57 PFLOP/s for some milliseconds (0.93 of the measured peak), 1.36 at 1.2 to 1.35 GHz; 4 bits, 8192 tokens, 4096 -> 8192, 104 us
+// (5.3 PFLOP/s), 118 to 123 at 1.5 GHz.  Short ones: about 5 us of launch, set-up and first copies, and a first tile's epilogue of 2,500 cycles (1,100
+// once its code is in the instruction cache); and this one width of tile, which leaves pairs idle where their number and the tiles' do not meet.
 #pragma once
 #include <type_traits>
 

@@ -10,13 +10,13 @@
 // accumulators (two a row quarter).  Few results: a cluster splits K and its CTAs' partial sums are added through distributed shared
 // memory in ascending rank order (no workspace, no atomics: the same bits on every run).
 //
-// What bounds it: the weights' bytes, and for the smallest the launch.  4-bit 65536 x 8192 (285 MB) 16 tokens 47.4 us (6.0 TB/s), 65536 x 4096 8 tokens 27.3
-// (5.2); gated bf16, 4 tokens, 4096 -> 10240 (168 MB) 31.2 (5.4; lower tiles that would share the weights evenly over the SMs change nothing); 4-bit
-// 4096 x 4096, one token, 5.3: 2.3 from the start to the first operands, 1.5 of products, 1.5 to join the parts and leave.
+// What bounds it: the weights' bytes, and for the smallest the launch.  4-bit 65536 x 8192 (285 MB) 16 tokens 47.4 us (6.0 TB/s), 65536 x 4096 8 tokens 26.3
+// (5.4); gated bf16, 4 tokens, 4096 -> 10240 (168 MB) 28.8 (5.8; lower tiles that would share the weights evenly over the SMs change nothing); 4-bit
+// 4096 x 4096, one token, 4.2 to 4.7 for the 1.4 that its bytes take: about half until the first operands are there, the rest products and the join.
 //
-// Up to 128 rows, as beyond that the other kernel's tiles are faster.  us a call here / there at 64, 96, 128 tokens: 4-bit 4096 x 4096 6.8 / 11.6, 7.8 / 11.8,
-// 8.1 / 11.9; 8192 -> 16384 18.6 / 19.8, 18.4 / 20.2, 19.6 / 20.5; gated bf16 4096 -> 10240 39 / 45, 44 / 45, 47 / 46; backward 2048 -> 5632 35 / 44, 35 /
-// 45, 37 / 46.  Accumulators for 16, 32, 64 or 128 rows, the fewest that hold them: up to 64, two blocks share an SM.
+// Up to 128 rows, as beyond that the other kernel's tiles are faster.  us a call here / there at 64, 96, 128 tokens: 4-bit 4096 x 4096 5.5 / 9.0, 6.9 / 9.3,
+// 7.3 / 9.6; 8192 -> 16384 17.5 / 17.6, 17.5 / 18.0, 18.6 / 18.3; gated bf16 4096 -> 10240 with pre 34.5 / 41.1, 42.6 / 42.3, 46.0 / 43.9; dx of
+// 2048 -> 5632, dg and du included, 14.9 / 22.7, 16.3 / 22.8, 18.4 / 22.7.  Accumulators for 16, 32, 64 or 128 rows, the fewest that hold them: up to 64, two blocks share an SM.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
